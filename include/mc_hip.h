@@ -19,7 +19,7 @@
 extern "C" {
 #endif
 
-#define MC_ABI_VERSION 10
+#define MC_ABI_VERSION 11
 
 /* activation codes for mc_gemm_bf16 */
 #define MC_ACT_NONE 0
@@ -392,6 +392,67 @@ int mc_sample_step_f32(const float* logits, int64_t ld, int64_t* next_ids, int64
 /* out[m][n] = logits[m][n] - logsumexp_n(logits[m]) (fp32): the scoring step of beam search (generate(num_beams > 1): transformers 4.31
  * beam_search, forwarded by eval/model_multimodal_qa_loader.py:94-102) */
 int mc_log_softmax_f32(const float* logits, int64_t ld, float* out, int64_t ldo, int M, int N, void* stream);
+
+/* Logits processor (csrc/logits.hip), before mc_argmax_f32 / mc_sample_step_f32; out may be logits (in place).  For row m, token t:
+ *   seen = t among the prompt or output ids, c = its number among the output ids
+ *   l = seen ? (l > 0 ? l / repetition[m] : l * repetition[m]) : l;   l -= frequency[m] * c + presence[m] * (c > 0);
+ *   l += sum of bias[m][i] over bias_ids[m][i] == t;   l = -inf unless bit t & 31 of allowed[m][t >> 5] is set.
+ * Every array but logits / out may be NULL: that part is left out (repetition 1, the penalties 0, no bias, everything allowed).  Ids outside
+ * [0, V) are ignored; lengths are clipped to [0, cols]; NULL lengths = cols.  All rows in row strides (elements). */
+typedef struct mc_logits_args {
+    const float* logits; int64_t ld; float* out; int64_t ld_out; int M, V;
+    const int64_t* prompt_ids; int64_t ld_prompt; const int32_t* prompt_lens; int prompt_cols;
+    const int64_t* output_ids; int64_t ld_output; const int32_t* output_lens; int output_cols;
+    const float* repetition; const float* presence; const float* frequency;   /* [M] each */
+    const int32_t* bias_ids; const float* bias; int64_t ld_bias; int n_bias;   /* [M, n_bias], n_bias <= 4096 */
+    const int32_t* allowed; int64_t ld_allowed;                               /* [M, ceil(V / 32)] */
+} mc_logits_args;
+int mc_logits_process_f32(const mc_logits_args* args, void* stream);
+
+/* ---- 4-bit weights (csrc/gemm_q4.hip) ------------------------------------------------------------------------------------------------
+ * W[n][k] = scales[n][k / group] * (code[n][k] - zeros[n][k / group]), codes 0..15.  codes: two to a byte, even k in the low half, row n at
+ * codes + n * ldc (bytes, 16-byte aligned rows); scales 16-bit, zeros uint8 (NULL: 8), row strides in elements.  group 32, 64 or 128, dividing K. */
+typedef struct mc_q4_weight {
+    const void* codes; int64_t ldc; const void* scales; int64_t lds; const void* zeros; int64_t ldz;
+    int N, K, group;
+} mc_q4_weight;
+/* out[M, N] = x[M, K] W^T (+ bias) (+ residual): at most 64 rows; out 16-bit, or fp32 with out_f32.  Codes are multiplied as exact integers and summed in
+ * fp32 per group, then scaled; a row's result does not depend on M. */
+int mc_linear_q4_bf16(const void* x, int64_t ldx, const mc_q4_weight* w, const void* bias, const void* residual, int64_t ldr, void* out, int64_t ldo,
+                      int M, int out_f32, void* stream);
+/* codes [N, K / 2], scales [N, K / group] (and zeros, unless NULL: symmetric codes around 8) of a 16-bit weight, all contiguous */
+int mc_quantize_q4_bf16(const void* w, int64_t ldw, void* codes, void* scales, void* zeros, int N, int K, int group, void* stream);
+/* the packed 16-bit form (mc_packed_weight_elems) for launches of more than 64 rows */
+int mc_dequantize_q4_bf16(const mc_q4_weight* w, void* packed, void* stream);
+
+/* ---- 8-bit KV cache (csrc/kv8.hip) -----------------------------------------------------------------------------------------------------
+ * One vector of D codes and one fp32 scale per (sequence, key head, position): scale = amax / T, code = rne(x * (T / amax)), amax = max(max |x|, 2^-100),
+ * T = 448 (MC_KV8_E4M3: OCP e4m3) or 127 (MC_KV8_INT8).  A vector with an infinity or NaN is stored as zero codes and a NaN scale.
+ * k / v: [B][Hkv][S][D] bytes with strides sb, sh, st (multiples of 16, head_dim contiguous), scales [B][Hkv][S] with strides scale_sb, scale_sh. */
+#define MC_KV8_E4M3 1
+#define MC_KV8_INT8 2
+typedef struct mc_kv8_cache {
+    void* k; float* k_scale; void* v; float* v_scale;
+    int64_t sb, sh, st, scale_sb, scale_sh;
+    int B, Hkv, S, D, format;
+} mc_kv8_cache;
+/* mc_rope_kv_bf16 for this cache: q rotated and stored 16-bit at q_out[(row_b Lq + row_t)][H D] (the same bits), k rotated in fp32 and quantised, v quantised, to
+ * position row_pos.  Rows with row_b < 0 (padding), or whose row_b / row_pos / row_t lies outside B / S and max_pos (rows of the tables) / Lq, write
+ * nothing.  No two rows may name the same position of the same sequence. */
+int mc_rope_kv8(const void* qkv, int64_t ld, const int32_t* row_b, const int32_t* row_pos, const int32_t* row_t, const float* cos_table,
+                const float* sin_table, int max_pos, void* q_out, const mc_kv8_cache* cache, int M, int H, int Lq, void* stream);
+/* k_out / v_out [B, Hkv, n, D] 16-bit = code * scale of the first n positions; positions >= kv_lens[b] (NULL: none) are zero rows */
+int mc_kv8_read(const mc_kv8_cache* cache, const int32_t* kv_lens, int n, void* k_out, void* v_out, void* stream);
+/* Decode attention (one query per sequence) over the first kv_lens[b] (clipped to S; NULL: S) keys; key_valid as in mc_attn_mask.  A sequence without a
+ * key gives a zero row.  A row's bits depend neither on B nor on S (chunks of keys at fixed positions, combined in order). */
+int mc_attn_decode8_workspace_bytes(int B, int H, int D, int S, int64_t* bytes);
+int mc_attn_decode8(const void* q, int64_t q_sb, int64_t q_sh, const mc_kv8_cache* cache, const int32_t* kv_lens, const void* key_valid,
+                    int64_t key_valid_stride, void* o, int64_t o_sb, void* workspace, int H, float scale, void* stream);
+/* with rotation and append: qkv [B, (H + 2 Hkv) D] pre-rotary, kv_lens counts this token, which is quantised to position kv_lens[b] - 1 and attended as stored.
+ * A sequence with kv_lens[b] < 1, > S or > max_pos is left alone: nothing is written and its output row is zero. */
+int mc_attn_decode8_rope(const void* qkv, int64_t qkv_ld, const float* cos_table, const float* sin_table, int max_pos, const mc_kv8_cache* cache,
+                         const int32_t* kv_lens, const void* key_valid, int64_t key_valid_stride, void* o, int64_t o_sb, void* workspace, int H,
+                         float scale, void* stream);
 
 /* ---- checkpoint files (csrc/ckpt_reader.cpp) --------------------------------------------------------------------------------
  * Replaces torch.load / safetensors in load_pretrained_model (model/builder.py:148, :157-168): adapter_model.bin, non_lora_trainables.bin,

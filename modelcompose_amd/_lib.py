@@ -12,7 +12,7 @@ LIB_PATH = os.path.join(_HERE, "libmc_hip.so")
 LIB_PATHS = {"bf16": LIB_PATH, "fp16": os.path.join(_HERE, "libmc_hip_f16.so")}
 if os.environ.get("MC_PROBES_LIB", "0") == "1":      # the probes build (bf16 only): tools/probes/*.py
     LIB_PATHS["bf16"] = LIB_PATH = os.path.join(os.path.dirname(_HERE), "tools", "probes", "libmc_hip_probes.so")
-ABI_VERSION = 10
+ABI_VERSION = 11
 _DTYPE_CODES = {"bf16": 1, "fp16": 2}                        # MC_DTYPE_BF16 / MC_DTYPE_F16 of mc_hip.h
 
 
@@ -154,7 +154,36 @@ class LlmConfigC(C.Structure):
                                        "max_pos")] + [("rms_eps", C.c_float)]
 
 
+class LogitsArgsC(C.Structure):
+    """struct mc_logits_args (include/mc_hip.h)."""
+    _fields_ = [("logits", c_p), ("ld", c_l), ("out", c_p), ("ld_out", c_l), ("M", c_i), ("V", c_i),
+                ("prompt_ids", c_p), ("ld_prompt", c_l), ("prompt_lens", c_p), ("prompt_cols", c_i),
+                ("output_ids", c_p), ("ld_output", c_l), ("output_lens", c_p), ("output_cols", c_i),
+                ("repetition", c_p), ("presence", c_p), ("frequency", c_p),
+                ("bias_ids", c_p), ("bias", c_p), ("ld_bias", c_l), ("n_bias", c_i), ("allowed", c_p), ("ld_allowed", c_l)]
+
+
+class Q4WeightC(C.Structure):
+    """struct mc_q4_weight (include/mc_hip.h)."""
+    _fields_ = [("codes", c_p), ("ldc", c_l), ("scales", c_p), ("lds", c_l), ("zeros", c_p), ("ldz", c_l), ("N", c_i), ("K", c_i), ("group", c_i)]
+
+
+class Kv8CacheC(C.Structure):
+    """struct mc_kv8_cache (include/mc_hip.h)."""
+    _fields_ = [("k", c_p), ("k_scale", c_p), ("v", c_p), ("v_scale", c_p), ("sb", c_l), ("sh", c_l), ("st", c_l), ("scale_sb", c_l), ("scale_sh", c_l),
+                ("B", c_i), ("Hkv", c_i), ("S", c_i), ("D", c_i), ("format", c_i)]
+
+
 _SIGS.update({
+    "mc_logits_process_f32": [C.POINTER(LogitsArgsC), c_p],
+    "mc_linear_q4_bf16": [c_p, c_l, C.POINTER(Q4WeightC), c_p, c_p, c_l, c_p, c_l, c_i, c_i, c_p],
+    "mc_quantize_q4_bf16": [c_p, c_l, c_p, c_p, c_p, c_i, c_i, c_i, c_p],
+    "mc_dequantize_q4_bf16": [C.POINTER(Q4WeightC), c_p, c_p],
+    "mc_rope_kv8": [c_p, c_l, c_p, c_p, c_p, c_p, c_p, c_i, c_p, C.POINTER(Kv8CacheC), c_i, c_i, c_i, c_p],
+    "mc_kv8_read": [C.POINTER(Kv8CacheC), c_p, c_i, c_p, c_p, c_p],
+    "mc_attn_decode8_workspace_bytes": [c_i, c_i, c_i, c_i, C.POINTER(c_l)],
+    "mc_attn_decode8": [c_p, c_l, c_l, C.POINTER(Kv8CacheC), c_p, c_p, c_l, c_p, c_l, c_p, c_i, c_f, c_p],
+    "mc_attn_decode8_rope": [c_p, c_l, c_p, c_p, c_i, C.POINTER(Kv8CacheC), c_p, c_p, c_l, c_p, c_l, c_p, c_i, c_f, c_p],
     "mc_gemm_ex_bf16": [C.POINTER(GemmArgsC), c_p],
     "mc_fbank_f32": [c_p, c_p, c_l, c_i, c_p, c_p, c_p, c_p, c_f, c_f, c_f, c_p, c_p, c_i, c_p],
     "mc_image_preprocess_u8": [c_p, c_i, c_i, c_i, c_i, c_i, c_i, C.POINTER(C.c_int32), c_p, c_p, c_i, c_p, c_p, c_i, c_i, c_i, c_i, c_i, c_i, c_i,

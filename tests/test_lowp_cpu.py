@@ -1,0 +1,117 @@
+"""Refusals of the low-precision serving operators: bad arguments are turned into errors before any launch (C ABI and Python wrappers)."""
+import ctypes as C
+
+import pytest
+import torch
+
+
+@pytest.fixture(scope="module")
+def lib():
+    import os
+    import __graft_entry__ as g
+    from modelcompose_amd import _lib
+    if not os.path.exists(_lib.LIB_PATH):
+        g.build()
+    return _lib
+
+
+def refused(lib, rc, text):
+    msg = lib.lib().mc_last_error().decode()
+    assert rc == 1 and text in msg, (rc, msg)
+    with pytest.raises(ValueError):
+        lib.check(rc, "call")
+
+
+def cache_c(lib, **kw):
+    d = dict(k=4096, k_scale=4096, v=4096, v_scale=4096, sb=1 << 20, sh=1 << 16, st=128, scale_sb=1024, scale_sh=128, B=2, Hkv=2, S=128, D=128, format=1)
+    d.update(kw)
+    return lib.Kv8CacheC(*[d[n] for n, _ in lib.Kv8CacheC._fields_])
+
+
+@pytest.mark.parametrize("bad,text", [(dict(k=0), "null cache"), (dict(v_scale=0), "null cache"), (dict(format=3), "format"), (dict(D=96), "head_dim"), (dict(S=0), "bad cache shape"),
+                                      (dict(B=-1), "bad cache shape"), (dict(st=72), "16-byte"), (dict(k=4100), "16-byte"), (dict(k_scale=4097), "4-byte"),
+                                      (dict(B=1 << 13, Hkv=1 << 12), "too large")])
+def test_bad_caches(lib, bad, text):
+    L, c = lib.lib(), cache_c(lib, **bad)
+    one = 4096
+    refused(lib, L.mc_kv8_read(C.byref(c), None, 1, one, one, None), text)
+    refused(lib, L.mc_rope_kv8(one, 1024, one, one, one, one, one, 16, one, C.byref(c), 1, 4, 1, None), text)
+    refused(lib, L.mc_attn_decode8(one, 512, 128, C.byref(c), None, None, 0, one, 512, one, 4, 1.0, None), text)
+    refused(lib, L.mc_attn_decode8_rope(one, 1024, one, one, 16, C.byref(c), one, None, 0, one, 512, one, 4, 1.0, None), text)
+
+
+def test_bad_cache_calls(lib):
+    L, c, one = lib.lib(), C.byref(cache_c(lib)), 4096
+    refused(lib, L.mc_kv8_read(c, None, 129, one, one, None), "129 positions")
+    refused(lib, L.mc_kv8_read(c, None, 1, None, one, None), "null")
+    refused(lib, L.mc_kv8_read(c, None, 1, one, 4104, None), "misaligned")
+    refused(lib, L.mc_rope_kv8(one, 1024, one, one, one, one, one, 16, one, c, 1, 3, 1, None), "3 query heads over 2")
+    refused(lib, L.mc_rope_kv8(one, 1016, one, one, one, one, one, 16, one, c, 1, 4, 1, None), "qkv rows")
+    refused(lib, L.mc_rope_kv8(one, 1028, one, one, one, one, one, 16, one, c, 1, 4, 1, None), "qkv rows")
+    refused(lib, L.mc_rope_kv8(one, 1024, one, None, one, one, one, 16, one, c, 1, 4, 1, None), "null")
+    refused(lib, L.mc_rope_kv8(one, 1024, one, one, one, one, one, 0, one, c, 1, 4, 1, None), "tables")
+    refused(lib, L.mc_rope_kv8(one, 1024, one, one, one, one, one, 16, one, c, 1, 4, 0, None), "bad shape")
+    refused(lib, L.mc_rope_kv8(one, 1024, one, one, one, one, one, 16, one, c, 1 << 30, 4, 1, None), "too many rows")
+    assert L.mc_rope_kv8(one, 1024, one, one, one, one, one, 16, one, c, 0, 4, 1, None) == 0          # no rows: no launch
+    refused(lib, L.mc_attn_decode8(one, 512, 128, c, None, None, 0, one, 512, None, 4, 1.0, None), "null")
+    refused(lib, L.mc_attn_decode8(one, 516, 128, c, None, None, 0, one, 512, one, 4, 1.0, None), "16-byte")
+    refused(lib, L.mc_attn_decode8(one, 512, 128, c, None, None, 0, one, 512, one, 5, 1.0, None), "5 query heads")
+    refused(lib, L.mc_attn_decode8_rope(one, 1024, one, one, 16, c, None, None, 0, one, 512, one, 4, 1.0, None), "null")
+    n = C.c_int64(0)
+    refused(lib, L.mc_attn_decode8_workspace_bytes(0, 1, 128, 1, C.byref(n)), "bad arguments")
+
+
+def test_bad_q4_calls(lib):
+    L, one = lib.lib(), 4096
+
+    def w(**kw):
+        d = dict(codes=4096, ldc=128, scales=4096, lds=2, zeros=0, ldz=0, N=8, K=256, group=128)
+        d.update(kw)
+        return lib.Q4WeightC(*[d[n] for n, _ in lib.Q4WeightC._fields_])
+    call = lambda ww, M=4, ldx=256, x=one, ldo=8, out=one: L.mc_linear_q4_bf16(x, ldx, C.byref(ww), None, None, 0, out, ldo, M, 0, None)
+    for bad, text in ((dict(codes=0), "null weight"), (dict(group=96), "group 96"), (dict(K=192), "multiple"), (dict(N=0), "positive"), (dict(ldc=120), "16-byte"), (dict(ldc=112), "16-byte"),
+                      (dict(codes=4100), "16-byte"), (dict(lds=1), "scales or zeros"), (dict(zeros=4096, ldz=1), "scales or zeros")):
+        refused(lib, call(w(**bad)), text)
+        refused(lib, L.mc_dequantize_q4_bf16(C.byref(w(**bad)), one, None), text)
+    refused(lib, call(w(), M=65), "at most 64")
+    refused(lib, call(w(), M=-1), "at most 64")
+    refused(lib, call(w(), ldx=252), "rows of x")
+    refused(lib, call(w(), ldx=248), "rows of x")
+    refused(lib, call(w(), x=None), "rows of x")
+    refused(lib, call(w(), ldo=7), "bad output")
+    assert call(w(), M=0) == 0
+    refused(lib, L.mc_dequantize_q4_bf16(C.byref(w()), None, None), "null")
+    refused(lib, L.mc_quantize_q4_bf16(one, 256, one, one, None, 8, 200, 128, None), "dividing K")
+    refused(lib, L.mc_quantize_q4_bf16(one, 250, one, one, None, 8, 256, 128, None), "16-byte")
+    refused(lib, L.mc_quantize_q4_bf16(None, 256, one, one, None, 8, 256, 128, None), "null")
+
+
+def test_bad_logits_calls(lib):
+    L = lib.lib()
+    call = lambda **kw: L.mc_logits_process_f32(C.byref(lib.LogitsArgsC(**{**dict(logits=4096, out=4096, ld=8, ld_out=8, M=2, V=8), **kw})), None)
+    refused(lib, call(logits=0), "null")
+    refused(lib, call(V=0), "bad shape")
+    refused(lib, call(M=-1), "bad shape")
+    refused(lib, call(ld=7), "rows overlap")
+    refused(lib, call(prompt_ids=4096, prompt_cols=-1), "negative")
+    refused(lib, call(bias_ids=4096, bias=0, n_bias=2), "biases")
+    refused(lib, call(bias_ids=4096, bias=4096, n_bias=4097), "biases")
+    assert call(M=0) == 0
+
+
+def test_wrappers_refuse_host_tensors():
+    from modelcompose_amd import ops
+    z = torch.zeros
+    st = ops.BF16
+    with pytest.raises(ValueError, match="no CPU fallback"):
+        ops.Q4Weight(z(8, 64, dtype=torch.uint8), z(8, 1, dtype=st))
+    with pytest.raises(ValueError, match="no CPU fallback"):
+        ops.Kv8Cache(z(1, 1, 4, 64, dtype=torch.int8), z(1, 1, 4), z(1, 1, 4, 64, dtype=torch.int8), z(1, 1, 4))
+    with pytest.raises(ValueError, match="no CPU fallback"):
+        ops.logits_process(z(2, 8))
+    with pytest.raises(ValueError, match="device"):
+        ops.quantize_q4(z(8, 128, dtype=st))
+    with pytest.raises(ValueError, match="no CPU fallback"):
+        ops.linear_q4(z(1, 64, dtype=st), None)
+    with pytest.raises(ValueError, match="no CPU fallback"):
+        ops.attn_decode8(z(1, 1, 64, dtype=st), None)

@@ -1,0 +1,660 @@
+"""Low-precision serving operators (csrc/gemm_q4.hip, csrc/kv8.hip, csrc/logits.hip) against plain 64-bit implementations on the CPU.
+
+Tolerances: a 16-bit output is off by at most half a step of the storage dtype (eps / 2 relative) plus the fp32 error of what is summed, bounded per
+element from the terms' magnitudes (the comment at each bound); integer outputs and codes are equal."""
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+FMTS = {"e4m3": torch.float8_e4m3fn, "int8": torch.int8}
+TOP = {"e4m3": 448.0, "int8": 127.0}
+U = 2.0 ** -24                                             # fp32: half a step
+
+
+@pytest.fixture(scope="module", autouse=True)
+def _gpu():
+    if not torch.cuda.is_available():
+        pytest.skip("needs a GPU")
+
+
+def _st():
+    from modelcompose_amd import ops
+    return ops.BF16
+
+
+def _half():
+    return torch.finfo(_st()).eps / 2
+
+
+def _gen(seed):
+    return torch.Generator().manual_seed(seed)
+
+
+def _rand(g, *shape):
+    return torch.randn(*shape, generator=g).to(_st())
+
+
+# ---- plain forms -----------------------------------------------------------------------------------------------------------------
+def quantise(x, fmt):
+    """fp32 [..., D] -> (codes, scale): the definition, operation by operation (CPU fp32 is IEEE: the codes must be equal bit for bit)."""
+    x = x.float()
+    amax = x.abs().amax(-1)
+    ok = torch.isfinite(amax)
+    amax = torch.where(ok, amax, torch.ones_like(amax)).clamp_min(2.0 ** -100)
+    inv = torch.full_like(amax, TOP[fmt]) / amax
+    y = torch.where(ok[..., None], x * inv[..., None], torch.zeros_like(x))
+    codes = y.to(torch.float8_e4m3fn) if fmt == "e4m3" else y.round().to(torch.int8)
+    return codes, torch.where(ok, amax * torch.tensor(1.0 / TOP[fmt], dtype=torch.float32), torch.full_like(amax, math.nan))
+
+
+def rotate(x, cos, sin):
+    """x [..., D] fp32, cos / sin broadcastable [..., D / 2]; products and sum rounded on their own."""
+    h = x.shape[-1] // 2
+    a, b = x[..., :h], x[..., h:]
+    return torch.cat([a * cos - b * sin, b * cos + a * sin], -1)
+
+
+def tables(n, D, theta=10000.0):
+    ang = torch.outer(torch.arange(n, dtype=torch.float64), 1.0 / theta ** (torch.arange(0, D, 2, dtype=torch.float64) / D))
+    return ang.cos().float(), ang.sin().float()
+
+
+def value(codes, scale):
+    return codes.float().double() * scale.double()[..., None]
+
+
+def make_cache(g, B, Hkv, S, D, fmt, layout="bhsd"):
+    """A cache of random vectors on the GPU -> (Kv8Cache, and on the CPU: k codes, k scale, v codes, v scale)."""
+    from modelcompose_amd import ops
+    host = []
+    for _ in range(2):
+        c, s = quantise(torch.randn(B, Hkv, S, D, generator=g), fmt)
+        host += [c, s]
+
+    def place(t):
+        u = t.view(torch.uint8) if t.dtype in (torch.float8_e4m3fn, torch.int8) else t
+        if layout == "bshd" and t.dim() == 4:                     # positions outside heads
+            return u.transpose(1, 2).contiguous().cuda().transpose(1, 2).view(t.dtype) if t.dtype == torch.int8 else \
+                u.transpose(1, 2).contiguous().cuda().view(t.dtype).transpose(1, 2)
+        return u.cuda().view(t.dtype) if t.dim() == 4 else u.cuda()
+    k, ks, v, vs = (place(t) for t in host)
+    return ops.Kv8Cache(k, ks, v, vs), host
+
+
+def attend(q, host, lens, scale, key_valid=None):
+    """(out, bound): softmax attention in 64 bits and what 16-bit storage and fp32 arithmetic may add.  q fp64 [B, H, D]."""
+    kc, ks, vc, vs = host
+    B, H, D = q.shape
+    Hkv = kc.shape[1]
+    out, bound = torch.zeros(B, H, D, dtype=torch.float64), torch.zeros(B, H, D, dtype=torch.float64)
+    for b in range(B):
+        at = torch.arange(max(0, min(int(lens[b]), kc.shape[2])))
+        if key_valid is not None:
+            at = at[key_valid[b, :len(at)] != 0]
+        if not len(at):
+            continue
+        for h in range(H):
+            hk = h // (H // Hkv)
+            k, v = value(kc[b, hk, at], ks[b, hk, at]), value(vc[b, hk, at], vs[b, hk, at])
+            p = torch.softmax(k @ q[b, h] * scale, 0)
+            out[b, h] = p @ v
+            # score: D fused or D separately rounded products of fp32, two scalings; the weights carry its absolute error as a relative one, doubled
+            # by the normalisation; n terms are summed, and each weight is held to 2^-17 or better
+            delta = (D + 4) * U * (k.abs() @ q[b, h].abs() * abs(scale)).max()
+            bound[b, h] = _half() * out[b, h].abs() + (2 * delta + (len(at) + 16) * 2 * U + 2.0 ** -16) * (p @ v.abs()) + 1e-30
+    return out, bound
+
+
+def near(got, ref, bound):
+    d = (got.double().cpu() - ref).abs()
+    assert torch.isfinite(got.float()).all()
+    assert (d <= bound * (1 + 1e-6)).all(), f"worst {float((d / bound.clamp_min(1e-300)).max())} of the bound"
+
+
+# ---- cache write and read-back -----------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("fmt", list(FMTS))
+@pytest.mark.parametrize("B,L,H,Hkv,D,layout", [(1, 1, 2, 2, 128, "bhsd"), (3, 37, 6, 2, 64, "bhsd"), (2, 65, 4, 4, 128, "bshd"), (2, 9, 17, 1, 64, "bshd")])
+def test_rope_kv8_and_read(fmt, B, L, H, Hkv, D, layout):
+    from modelcompose_amd import ops
+    g = _gen(1)
+    S = L + 3
+    lens = torch.tensor([max(1, L - 5 * b) for b in range(B)], dtype=torch.int32)
+    M = B * L
+    qkv = _rand(g, M, (H + 2 * Hkv) * D + 8)[:, :(H + 2 * Hkv) * D]                  # row stride wider than the row
+    order = torch.randperm(M, generator=g)
+    row_b, row_t = (order // L).int(), (order % L).int()
+    row_b[row_t >= lens[row_b.long()]] = -1
+    cos, sin = tables(S, D)
+    cache, host = make_cache(g, B, Hkv, S, D, fmt, layout)
+    before = [t.clone() for t in host]
+    qs = qkv.stride(0)
+    dq = torch.empty(M, qs, dtype=_st(), device="cuda")[:, :qkv.shape[1]]
+    dq.copy_(qkv)
+    q_out = torch.full((B * L, H * D), 7.0, dtype=_st(), device="cuda")
+    ops.rope_kv8(dq, row_b.cuda(), row_t.cuda(), row_t.cuda(), cos.cuda(), sin.cuda(), q_out, cache, H, L)
+    # the 16-bit form's queries, bit for bit
+    q16 = torch.full((B * L, H * D), 7.0, dtype=_st(), device="cuda")
+    kc, vc = (torch.zeros(B, Hkv, S, D, dtype=_st(), device="cuda") for _ in range(2))
+    ops.rope_kv(dq, row_b.cuda(), row_t.cuda(), row_t.cuda(), cos.cuda(), sin.cuda(), q16, kc, vc, H, Hkv, D, L, S)
+    assert torch.equal(q_out, q16)
+    want = [t.clone() for t in before]
+    x = qkv.float().view(M, H + 2 * Hkv, D)
+    for r in range(M):
+        b, t = int(row_b[r]), int(row_t[r])
+        if b < 0:
+            continue
+        for i, y in ((0, rotate(x[r, H:H + Hkv], cos[t], sin[t])), (2, x[r, H + Hkv:])):
+            c, s = quantise(y, fmt)
+            want[i].view(torch.uint8)[b, :, t] = c.view(torch.uint8)
+            want[i + 1][b, :, t] = s
+            # half a code step of the exact value: e4m3 2^-4 of it, or 2^-10 scales among the subnormals; int8 half a scale
+            ref = y.double()
+            step = torch.maximum(ref.abs() * 2.0 ** -4, s.double()[:, None] * 2.0 ** -10) if fmt == "e4m3" else s.double()[:, None] * 0.5
+            assert ((value(c, s) - ref).abs() <= step * (1 + 1e-5)).all()
+    for got, ref in zip((cache.k, cache.k_scale, cache.v, cache.v_scale), want):
+        got = got.cpu()
+        assert torch.equal(got.view(torch.uint8) if got.dim() == 4 else got, ref.view(torch.uint8) if ref.dim() == 4 else ref)
+    for n in (L, S, 1, 0):
+        k, v = ops.kv8_read(cache, n, kv_lens=lens.cuda())
+        inside = (torch.arange(n) < lens[:, None])[:, None, :, None]
+        for got, i in ((k, 0), (v, 2)):
+            assert torch.equal(got.cpu(), torch.where(inside, want[i][:, :, :n].float() * want[i + 1][:, :, :n, None], torch.tensor(0.0)).to(_st()))
+    k, _ = ops.kv8_read(cache)
+    assert torch.equal(k.cpu(), (want[0].float() * want[1][..., None]).to(_st()))
+
+
+@pytest.mark.parametrize("fmt", list(FMTS))
+def test_special_vectors(fmt):
+    """Zero, tiny, huge and non-finite vectors; an infinity or NaN stays in its own vector."""
+    from modelcompose_amd import ops
+    D, S = 64, 8
+    qkv = torch.zeros(S, 3 * D, dtype=torch.float32)
+    for r, x in enumerate((0.0, torch.finfo(_st()).tiny, torch.finfo(_st()).max / 4, 1.0, 2.0, 3.0, 4.0, 5.0)):
+        qkv[r] = x
+    qkv[4, 2 * D + 3], qkv[5, 2 * D + 7], qkv[6, 2 * D + 9] = math.inf, math.nan, -math.inf
+    qkv = qkv.to(_st())
+    cos, sin = torch.ones(S, D // 2), torch.zeros(S, D // 2)
+    cache = ops.kv8_cache(1, 1, S, D, dtype=FMTS[fmt])
+    i32 = lambda t: torch.as_tensor(t, dtype=torch.int32).cuda()
+    q = torch.zeros(S, D, dtype=_st(), device="cuda")
+    ops.rope_kv8(qkv.cuda(), i32([0] * S), i32(range(S)), i32(range(S)), cos.cuda(), sin.cuda(), q, cache, 1, S)
+    for name, part in (("k", qkv[:, D:2 * D]), ("v", qkv[:, 2 * D:])):
+        c, s = quantise(part, fmt)
+        assert torch.equal(getattr(cache, name)[0, 0].cpu().view(torch.uint8), c.view(torch.uint8))
+        assert torch.equal(torch.nan_to_num(getattr(cache, name + "_scale")[0, 0].cpu(), nan=-1.0), torch.nan_to_num(s, nan=-1.0))
+    _, v = ops.kv8_read(cache)
+    assert torch.isnan(v[0, 0, 4:7]).all() and torch.isfinite(v[0, 0, :4]).all() and torch.isfinite(v[0, 0, 7]).all()
+    # masked or beyond the length they touch nothing; attended they make the row NaN
+    keep = torch.ones(1, S, dtype=torch.uint8)
+    keep[0, 4:7] = 0
+    qq = torch.ones(1, 1, D, dtype=_st(), device="cuda") * 0.01
+    assert torch.isfinite(ops.attn_decode8(qq, cache, kv_lens=i32([4]))).all()
+    assert torch.isfinite(ops.attn_decode8(qq, cache, key_valid=keep.cuda())).all()
+    assert torch.isnan(ops.attn_decode8(qq, cache)).all()
+
+
+def test_rows_outside_write_nothing():
+    from modelcompose_amd import ops
+    D, S, H = 64, 6, 2
+    cache = ops.kv8_cache(2, 1, S, D)
+    g = _gen(3)
+    qkv = _rand(g, 7, (H + 2) * D).cuda()
+    i32 = lambda *t: torch.tensor(t, dtype=torch.int32).cuda()
+    cos, sin = (t.cuda() for t in tables(5, D))                      # one row less than the cache
+    q = torch.full((2 * 3, H * D), 3.0, dtype=_st(), device="cuda")
+    #            padding  past B   pos < 0  past S   past tables  t past Lq  good
+    ops.rope_kv8(qkv, i32(-1, 2, 0, 0, 0, 0, 1), i32(0, 0, -1, 6, 5, 1, 4), i32(0, 0, 0, 0, 0, 3, 2), cos, sin, q, cache, H, 3)
+    ks = cache.k_scale.cpu()
+    assert ks[1, 0, 4] > 0 and int((ks != 0).sum()) == 1 and int((cache.v_scale != 0).sum()) == 1
+    q = q.cpu()
+    assert (q[:5] == 3.0).all() and not (q[5] == 3.0).all()
+    ops.rope_kv8(qkv[:0], i32(), i32(), i32(), cos, sin, q.cuda(), cache, H, 3)          # no rows: nothing happens
+
+
+# ---- decode attention ----------------------------------------------------------------------------------------------------------------
+SHAPES = [(1, 1, 1, 1, 128), (1, 2, 2, 31, 128), (2, 8, 8, 33, 64), (3, 6, 2, 130, 128), (2, 16, 2, 517, 64), (2, 12, 1, 700, 128), (1, 32, 2, 1100, 128),
+          (5, 4, 4, 1025, 64), (2, 3, 1, 2100, 128), (1, 24, 1, 513, 64)]
+
+
+@pytest.mark.parametrize("fmt", list(FMTS))
+@pytest.mark.parametrize("B,H,Hkv,S,D", SHAPES)
+def test_attn_decode8(fmt, B, H, Hkv, S, D):
+    from modelcompose_amd import ops
+    g = _gen(B * 1000 + S)
+    cache, host = make_cache(g, B, Hkv, S, D, fmt, "bshd" if B == 2 else "bhsd")
+    q = _rand(g, B, H, D)
+    lens = torch.tensor([S - (b * 37) % S for b in range(B)], dtype=torch.int32)
+    scale = 1.0 / math.sqrt(D)
+    ref, bound = attend(q.double(), host, lens, scale)
+    got = ops.attn_decode8(q.cuda(), cache, kv_lens=lens.cuda()).view(B, H, D)
+    near(got, ref, bound)
+    got = ops.attn_decode8(q.cuda(), cache, scale=3.0 * scale).view(B, H, D)               # every position; a sharper softmax
+    near(got, *attend(q.double(), host, [S] * B, 3.0 * scale))
+    keep = (torch.rand(B, S + 5, generator=g) < 0.7)
+    keep[:, :min(S - 1, S // 3)] = False
+    keep[0] = False                                                                       # a row that is left with nothing
+    keep[-1, S // 2:] = True
+    ref, bound = attend(q.double(), host, lens, scale, keep)
+    got = ops.attn_decode8(q.cuda(), cache, kv_lens=lens.cuda(), key_valid=keep.cuda()).view(B, H, D)
+    near(got, ref, bound)
+    if B > 1:
+        assert (got[0] == 0).all()
+
+
+@pytest.mark.parametrize("fmt", list(FMTS))
+def test_lengths_of_zero_and_garbage_behind_the_end(fmt):
+    """Lengths 0, negative, one, S and past S; whatever lies behind a length - codes that are no numbers, NaN and infinite scales - is never felt."""
+    from modelcompose_amd import ops
+    g = _gen(11)
+    B, H, Hkv, S, D = 6, 4, 2, 600, 128
+    cache, host = make_cache(g, B, Hkv, S, D, fmt)
+    lens = torch.tensor([0, -3, 1, S, S + 9, 577], dtype=torch.int32)
+    for b in range(B):
+        n = max(0, int(lens[b]))
+        cache.k[b, :, n:].view(torch.uint8).fill_(0xFF)
+        cache.v[b, :, n:].view(torch.uint8).fill_(0x7F)
+        cache.k_scale[b, :, n:] = math.nan
+        cache.v_scale[b, :, n:] = math.inf
+    q = _rand(g, B, H, D)
+    ref, bound = attend(q.double(), host, lens, 1 / math.sqrt(D))
+    out = torch.full((B, H * D + 8), 5.0, dtype=_st(), device="cuda")
+    got = ops.attn_decode8(q.cuda(), cache, kv_lens=lens.cuda(), out=out[:, :H * D])
+    near(got.reshape(B, H, D), ref, bound)
+    assert (got[:2] == 0).all() and (out[:, H * D:] == 5.0).all()
+    # the same poison at masked keys inside the length
+    cache, host = make_cache(g, 1, Hkv, S, D, fmt)
+    keep = torch.rand(1, S, generator=g) < 0.5
+    hit = (~keep[0]).nonzero()[:, 0].cuda()
+    cache.k.view(torch.uint8)[0, :, hit] = 0xFF
+    cache.v.view(torch.uint8)[0, :, hit] = 0xFF
+    cache.k_scale[0, :, hit], cache.v_scale[0, :, hit] = math.inf, math.nan
+    near(ops.attn_decode8(q[:1].cuda(), cache, key_valid=keep.cuda()).view(1, H, D), *attend(q[:1].double(), host, [S], 1 / math.sqrt(D), keep))
+
+
+def test_extreme_scores():
+    """Scores of thousands with either sign: the running maximum has to carry them, also where the first keys are far below the last."""
+    from modelcompose_amd import ops
+    g = _gen(12)
+    B, H, S, D = 2, 2, 1200, 64
+    cache, host = make_cache(g, B, H, S, D, "e4m3")
+    host[1].mul_(torch.linspace(0.0, 60.0, S))
+    cache.k_scale.copy_(host[1])
+    q = _rand(g, B, H, D) * 4
+    q[1] = -q[1]
+    ref, bound = attend(q.double(), host, [S] * B, 1.0)
+    near(ops.attn_decode8(q.cuda(), cache, scale=1.0).view(B, H, D), ref, bound)
+
+
+@pytest.mark.parametrize("fmt", list(FMTS))
+@pytest.mark.parametrize("B,H,Hkv,S,D", [(1, 2, 2, 64, 128), (4, 6, 2, 530, 64), (3, 32, 32, 1027, 128), (2, 9, 1, 40, 128)])
+def test_attn_decode8_rope_is_append_then_attend(fmt, B, H, Hkv, S, D):
+    from modelcompose_amd import ops
+    g = _gen(21)
+    cache, host = make_cache(g, B, Hkv, S, D, fmt)
+    lens = torch.tensor([1, S, S // 2 + 1, S - 1][:B], dtype=torch.int32)
+    qkv = _rand(g, B, (H + 2 * Hkv) * D)
+    cos, sin = tables(S, D)
+    out = ops.attn_decode8_rope(qkv.cuda(), cos.cuda(), sin.cuda(), cache, lens.cuda(), H)
+    x = qkv.float().view(B, H + 2 * Hkv, D)
+    q = torch.empty(B, H, D, dtype=torch.float64)
+    q16 = torch.zeros(B, H * D, dtype=_st(), device="cuda")
+    i32 = lambda t: torch.as_tensor(t, dtype=torch.int32).cuda()
+    trash = [torch.zeros(B, Hkv, S, D, dtype=_st(), device="cuda") for _ in range(2)]
+    ops.rope_kv(qkv.cuda(), i32(range(B)), i32(lens - 1), i32([0] * B), cos.cuda(), sin.cuda(), q16, *trash, H, Hkv, D, 1, S)
+    q = q16.cpu().double().view(B, H, D)
+    for b in range(B):
+        t = int(lens[b]) - 1
+        for i, y in ((0, rotate(x[b, H:H + Hkv], cos[t], sin[t])), (2, x[b, H + Hkv:])):
+            c, s = quantise(y, fmt)
+            host[i].view(torch.uint8)[b, :, t] = c.view(torch.uint8)
+            host[i + 1][b, :, t] = s
+    for got, ref in zip((cache.k, cache.k_scale, cache.v, cache.v_scale), host):
+        got = got.cpu()
+        assert torch.equal(got.view(torch.uint8) if got.dim() == 4 else got, ref.view(torch.uint8) if ref.dim() == 4 else ref)
+    near(out.view(B, H, D), *attend(q, host, lens, 1 / math.sqrt(D)))
+    # the append and the attention over the appended cache give the same bits as the two calls
+    assert torch.equal(out, ops.attn_decode8(q16.view(B, H, D), cache, kv_lens=lens.cuda()))
+    keep = torch.rand(B, S, generator=g) < 0.6
+    got = ops.attn_decode8_rope(qkv.cuda(), cos.cuda(), sin.cuda(), cache, lens.cuda(), H, key_valid=keep.cuda())
+    near(got.view(B, H, D), *attend(q, host, lens, 1 / math.sqrt(D), keep))
+
+
+def test_attn_decode8_rope_leaves_idle_sequences_alone():
+    from modelcompose_amd import ops
+    g = _gen(22)
+    B, H, S, D = 5, 2, 48, 64
+    cache, host = make_cache(g, B, H, S, D, "int8")
+    cos, sin = tables(40, D)                                                           # fewer rows than the cache has positions
+    lens = torch.tensor([0, S + 1, 41, 40, -7], dtype=torch.int32)
+    out = torch.full((B, H * D), 9.0, dtype=_st(), device="cuda")
+    ops.attn_decode8_rope(_rand(g, B, 3 * H * D).cuda(), cos.cuda(), sin.cuda(), cache, lens.cuda(), H, out=out)
+    assert (out[[0, 1, 2, 4]] == 0).all() and (out[3] != 0).any()
+    for b in (0, 1, 2, 4):
+        assert torch.equal(cache.k[b].cpu(), host[0][b]) and torch.equal(cache.v_scale[b].cpu(), host[3][b])
+
+
+def test_a_row_does_not_depend_on_its_batch_or_the_cache_size():
+    from modelcompose_amd import ops
+    g = _gen(23)
+    H, Hkv, S, D = 8, 2, 1500, 128
+    cache, host = make_cache(g, 40, Hkv, S, D, "e4m3")
+    q = _rand(g, 40, H, D).cuda()
+    lens = torch.randint(1, S + 1, (40,), generator=g).int()
+    whole = ops.attn_decode8(q, cache, kv_lens=lens.cuda())
+    for b0, b1 in ((0, 1), (7, 11), (39, 40)):
+        sub = ops.Kv8Cache(cache.k[b0:b1], cache.k_scale[b0:b1], cache.v[b0:b1], cache.v_scale[b0:b1])
+        assert torch.equal(ops.attn_decode8(q[b0:b1], sub, kv_lens=lens[b0:b1].cuda()), whole[b0:b1])
+    n = int(lens[7])                                                                    # a cache of exactly that many positions
+    sub = ops.Kv8Cache(cache.k[7:8, :, :n], cache.k_scale[7:8, :, :n], cache.v[7:8, :, :n], cache.v_scale[7:8, :, :n])
+    assert torch.equal(ops.attn_decode8(q[7:8], sub), whole[7:8])
+
+
+def test_offsets_past_32_bits():
+    """A cache of more than 2^31 bytes: written, read and attended at its far end."""
+    from modelcompose_amd import ops
+    Hkv, S, D = 2, (1 << 23) + 77, 128                                                   # 2 x 1.07e9 bytes: head 1 ends past 2^31
+    cache = ops.kv8_cache(1, Hkv, S, D, dtype=torch.int8)
+    g = _gen(31)
+    x = _rand(g, 1, 3 * Hkv * D)
+    cos, sin = torch.ones(1, D // 2), torch.zeros(1, D // 2)
+    i32 = lambda t: torch.as_tensor(t, dtype=torch.int32).cuda()
+    big_cos, big_sin = torch.ones(S, D // 2, device="cuda"), torch.zeros(S, D // 2, device="cuda")
+    q = torch.zeros(1, Hkv * D, dtype=_st(), device="cuda")
+    ops.rope_kv8(x.cuda(), i32([0]), i32([S - 1]), i32([0]), big_cos, big_sin, q, cache, Hkv, 1)
+    v = x.float().view(3 * Hkv, D)[2 * Hkv:]
+    c, s = quantise(v, "int8")
+    assert torch.equal(cache.v[0, :, S - 1].cpu(), c) and torch.equal(cache.v_scale[0, :, S - 1].cpu(), s)
+    assert int((cache.k_scale != 0).sum()) == Hkv
+    keep = torch.zeros(1, S, dtype=torch.uint8, device="cuda")
+    keep[0, S - 1] = 1
+    out = ops.attn_decode8(x[:, :Hkv * D].view(1, Hkv, D).cuda(), cache, key_valid=keep)
+    assert torch.equal(out.cpu().view(Hkv, D), (c.float() * s[:, None]).to(_st()))
+    _, vr = ops.kv8_read(cache)
+    assert torch.equal(vr[0, :, S - 1].cpu(), (c.float() * s[:, None]).to(_st())) and int((vr != 0).sum()) == int((vr[0, :, S - 1] != 0).sum())
+
+
+# ---- 4-bit weights ---------------------------------------------------------------------------------------------------------------------
+def q4_ref(x, codes, scales, zeros, group):
+    """(product, sum of the terms' magnitudes with the zero points counted on their own) in 64 bits."""
+    N = codes.shape[0]
+    q = torch.stack([codes & 15, codes >> 4], -1).view(N, -1).double()
+    z = 8.0 if zeros is None else zeros.double().repeat_interleave(group, 1)
+    s = scales.double().repeat_interleave(group, 1)
+    return x.double() @ ((q - z) * s).t().contiguous(), x.double().abs() @ ((q + z) * s.abs()).t().contiguous()
+
+
+def random_q4(g, N, K, group, zeros):
+    codes = torch.randint(0, 256, (N, K // 2), generator=g).to(torch.uint8)
+    scales = (torch.rand(N, K // group, generator=g) * 0.01 + 0.001).to(_st())
+    return codes, scales, torch.randint(0, 16, (N, K // group), generator=g).to(torch.uint8) if zeros else None
+
+
+@pytest.mark.parametrize("M", [1, 2, 15, 16, 17, 33, 48, 64])
+@pytest.mark.parametrize("N,K,group,zeros", [(1, 32, 32, False), (16, 128, 128, True), (17, 96, 32, True), (65, 1024, 64, False), (250, 4096, 128, True),
+                                             (33, 11008, 128, False), (129, 2752, 64, True), (40, 544, 32, False)])
+def test_linear_q4(M, N, K, group, zeros):
+    from modelcompose_amd import ops
+    g = _gen(N * 31 + M)
+    codes, scales, z = random_q4(g, N, K, group, zeros)
+    x, res, bias = _rand(g, M, K) + 0.25, _rand(g, M, N), _rand(g, N)                      # not centred: the zero points matter
+    w = ops.Q4Weight(codes.cuda(), scales.cuda(), None if z is None else z.cuda(), bias.cuda())
+    ref, mag = q4_ref(x, codes, scales, z, group)
+    err = (K + 16) * U * mag                                                               # K products summed in fp32 in whatever order, then scaled
+    y32 = ops.linear_q4(x.cuda(), w, out_f32=True, bias=False)
+    near(y32, ref, err + 1e-30)
+    y = ops.linear_q4(x.cuda(), w, residual=res.cuda())
+    full = ref + bias.double() + res.double()
+    near(y, full, _half() * full.abs() + err * 1.01 + 3 * U * (ref.abs() + bias.double().abs() + res.double().abs()) + 1e-30)
+    # strided rows in and out, and a row's bits in another batch
+    xs = torch.empty(M, K + 24, dtype=_st(), device="cuda")[:, :K]
+    xs.copy_(x)
+    out = torch.full((M, N + 3), 5.0, device="cuda")
+    assert torch.equal(ops.linear_q4(xs, w, out=out[:, :N], out_f32=True, bias=False), y32) and (out[:, N:] == 5.0).all()
+    assert torch.equal(ops.linear_q4(x[M // 2:M // 2 + 1].cuda(), w, out_f32=True, bias=False)[0], y32[M // 2])
+    res2 = res.cuda()
+    assert torch.equal(ops.linear_q4(x.cuda(), w, residual=res2, out=res2), y)               # the residual updated in place
+
+
+@pytest.mark.parametrize("symmetric", [True, False])
+@pytest.mark.parametrize("N,K,group", [(3, 32, 32), (37, 320, 64), (64, 1024, 128), (5, 4096, 128)])
+def test_quantize_and_dequantize_q4(N, K, group, symmetric):
+    from modelcompose_amd import ops
+    g = _gen(N + K)
+    w = _rand(g, N, K) * 0.02
+    w[0, :group] = 0
+    w[1, :group] = w[1, :group].abs()                                                       # one-sided groups
+    w[2, :group] = -w[2, :group].abs()
+    q = ops.quantize_q4(w.cuda(), group, symmetric)
+    assert (q.N, q.K, q.group) == (N, K, group)
+    v = w.float().view(N, K // group, group)
+    lo, hi = v.amin(-1).clamp_max(0), v.amax(-1).clamp_min(0)
+    s = (torch.maximum(hi, -lo) / 7 if symmetric else (hi - lo) / 15).to(_st())
+    assert torch.equal(q.scales.cpu(), s)
+    s = s.float()
+    z = torch.full_like(s, 8.0) if symmetric else torch.where(s > 0, (-lo / s).round(), torch.zeros_like(s)).clamp(0, 15)
+    if not symmetric:
+        assert torch.equal(q.zeros.cpu(), z.to(torch.uint8))
+    c = (torch.where(s[..., None] > 0, (v / s[..., None]).round(), torch.zeros_like(v)) + z[..., None]).clamp(0, 15)
+    codes = torch.stack([q.codes.cpu() & 15, q.codes.cpu() >> 4], -1).view(N, K // group, group).float()
+    assert torch.equal(codes, c)
+    # half a step from the weight, but for what the 16-bit scale leaves outside the range (8 steps times its half step)
+    assert ((codes - z[..., None]).double() * s.double()[..., None] - v.double()).abs().le(s.double()[..., None] * (0.5 + (16 * _half()) + 1e-6)).all()
+    pw = ops.dequantize_q4(q)
+    assert torch.equal(ops.unpack_weight(pw).cpu(), ((codes - z[..., None]) * s[..., None]).to(_st()).view(N, K))
+    wt = torch.empty(N, K + 8, dtype=_st(), device="cuda")[:, :K]
+    wt.copy_(w)
+    q2 = ops.quantize_q4(wt, group, symmetric)
+    assert torch.equal(q2.codes, q.codes) and torch.equal(q2.scales, q.scales)
+
+
+# ---- logits ----------------------------------------------------------------------------------------------------------------------------
+def logits_ref(x, prompt=None, plens=None, output=None, olens=None, rep=None, pres=None, freq=None, bids=None, bias=None, allowed=None):
+    """(processed, bound) in 64 bits, token by token."""
+    M, V = x.shape
+    y, mag = x.double().clone(), x.double().abs()
+    for m in range(M):
+        cut = lambda ids, lens: [] if ids is None else [int(t) for t in ids[m, :ids.shape[1] if lens is None else max(0, min(int(lens[m]), ids.shape[1]))] if 0 <= t < V]
+        old, new = cut(prompt, plens), cut(output, olens)
+        r = 1.0 if rep is None else float(rep[m])
+        for t in set(old + new):
+            y[m, t] = y[m, t] / r if y[m, t] > 0 else y[m, t] * r
+            mag[m, t] = y[m, t].abs()
+        for t in set(new):
+            d = (0.0 if freq is None else float(freq[m])) * new.count(t) + (0.0 if pres is None else float(pres[m]))
+            y[m, t] -= d
+            mag[m, t] += 2 * abs(d)
+        if bids is not None:
+            for i, t in enumerate(bids[m].tolist()):
+                if 0 <= t < V:
+                    y[m, t] += float(bias[m, i])
+                    mag[m, t] += bids.shape[1] * abs(float(bias[m, i]))
+        if allowed is not None:
+            bits = torch.tensor([(int(allowed[m, t >> 5]) >> (t & 31)) & 1 for t in range(V)], dtype=torch.bool)
+            y[m, ~bits] = -math.inf
+    return y, 4 * U * mag + 1e-38                             # at most 4 roundings of what has been added up so far, and the biases' own sum
+
+
+@pytest.mark.parametrize("M,V,Lp,Lo,nb", [(1, 1, 1, 1, 1), (3, 97, 40, 12, 5), (2, 2048, 300, 70, 0), (5, 2049, 1, 1, 9), (4, 5003, 700, 900, 33), (1, 32000, 50, 20, 8)])
+def test_logits_process(M, V, Lp, Lo, nb):
+    from modelcompose_amd import ops
+    g = _gen(V + M)
+    x = torch.randn(M, V, generator=g) * 4
+    prompt, output = (torch.randint(-3, V + 3, (M, L), generator=g) for L in (Lp, Lo))         # ids outside the vocabulary are ignored
+    prompt[0, 0] = -200
+    output[:, Lo // 2:] = output[:, :1]                                                       # one token many times
+    plens, olens = torch.randint(0, Lp + 1, (M,), generator=g).int(), torch.randint(0, Lo + 1, (M,), generator=g).int()
+    plens[-1], olens[0] = Lp + 5, -2                                                         # clipped
+    rep, pres, freq = 0.7 + torch.rand(M, generator=g), torch.randn(M, generator=g), torch.randn(M, generator=g)
+    bids = torch.randint(-2, V + 2, (M, nb), generator=g).int() if nb else None
+    bias = torch.randn(M, nb, generator=g) * 5 if nb else None
+    if nb > 2:
+        bids[:, 2] = bids[:, 0]                                                              # the same token twice
+    allowed = torch.randint(-2 ** 31, 2 ** 31, (M, (V + 31) // 32), generator=g).int()
+    cu = lambda t: None if t is None else t.cuda()
+    full = dict(prompt_ids=cu(prompt), prompt_lens=cu(plens), output_ids=cu(output), output_lens=cu(olens), repetition_penalty=cu(rep),
+                presence_penalty=cu(pres), frequency_penalty=cu(freq), bias_ids=cu(bids), bias=cu(bias), allowed=cu(allowed))
+
+    def check(got, ref, bound):
+        got = got.double().cpu()
+        assert torch.equal(torch.isinf(got), torch.isinf(ref)) and not torch.isnan(got).any()
+        fin = torch.isfinite(ref)
+        assert ((got - ref).abs()[fin] <= bound[fin]).all()
+    check(ops.logits_process(x.cuda(), **full), *logits_ref(x, prompt, plens, output, olens, rep, pres, freq, bids, bias, allowed))
+    check(ops.logits_process(x.cuda(), prompt_ids=cu(prompt), repetition_penalty=cu(rep)), *logits_ref(x, prompt, rep=rep))
+    check(ops.logits_process(x.cuda(), output_ids=cu(output), frequency_penalty=cu(freq)), *logits_ref(x, output=output, freq=freq))
+    assert torch.equal(ops.logits_process(x.cuda()).cpu(), x)
+    # rows with a stride, in place
+    xs = torch.full((M, V + 1), 3.0, device="cuda")
+    xs[:, :V] = x.cuda()
+    want = ops.logits_process(x.cuda(), **full)
+    assert torch.equal(ops.logits_process(xs[:, :V], out=xs[:, :V], **full), want) and (xs[:, V] == 3.0).all()
+
+
+def test_logits_process_special_values():
+    from modelcompose_amd import ops
+    x = torch.tensor([[math.inf, -math.inf, 0.0, -0.0, 1e38, -1e38, 5.0, math.nan]])
+    ids = torch.arange(8)[None]
+    y = ops.logits_process(x.cuda(), prompt_ids=ids.cuda(), repetition_penalty=torch.tensor([2.0]).cuda()).cpu()
+    assert y[0, :7].tolist() == [math.inf, -math.inf, 0.0, -0.0, float(torch.tensor(5e37)), float(torch.tensor(-2e38)), 2.5] and math.isnan(y[0, 7])
+    none = torch.zeros(1, 1, dtype=torch.int32).cuda()                                       # a mask that leaves nothing
+    assert torch.isneginf(ops.logits_process(x[:, :7].cuda(), allowed=none)).all()
+
+
+# ---- together ----------------------------------------------------------------------------------------------------------------------------
+class _Step:
+    """One decoder layer's decode step as a serving loop runs it, on low-precision weights and cache, then the next token."""
+
+    def __init__(self, seed, B=3, H=4, Hkv=2, D=64, S=80, V=1003):
+        from modelcompose_amd import ops
+        g = _gen(seed)
+        hid = H * D
+        self.dims = (B, H, Hkv, D, S, V)
+        self.w = {n: ops.quantize_q4((_rand(g, N, K) * 0.05).cuda(), 32, sym) for n, N, K, sym in (
+            ("qkv", (H + 2 * Hkv) * D, hid, True), ("o", hid, hid, False), ("lm", V, hid, False))}
+        self.cos, self.sin = (t.cuda() for t in tables(S, D))
+        self.embed = _rand(g, V, hid).cuda()
+        self.cache = ops.kv8_cache(B, Hkv, S, D)
+        self.lens = torch.tensor([5, 0, 17][:B], dtype=torch.int32).cuda()
+        n = 17
+        x = self.embed[torch.randint(0, V, (B * n,), generator=g).cuda()]
+        row = torch.arange(B * n)
+        b, t = (row // n).int(), (row % n).int()
+        b[t >= self.lens.cpu()[b.long()]] = -1
+        self.q = torch.zeros(B * n, hid, dtype=_st(), device="cuda")
+        ops.rope_kv8(ops.linear_q4(x, self.w["qkv"]), b.cuda(), t.cuda(), t.cuda(), self.cos, self.sin, self.q, self.cache, H, n)
+        self.ids = torch.randint(0, V, (B,), generator=g).cuda()
+        self.hist = torch.full((B, S), -1, dtype=torch.int64, device="cuda")
+        self.count = torch.zeros(B, dtype=torch.int32, device="cuda")
+        self.rep = torch.full((B,), 1.3, device="cuda")
+        self.freq = torch.full((B,), 0.4, device="cuda")
+
+    def __call__(self):
+        from modelcompose_amd import ops
+        B, H = self.dims[:2]
+        self.lens.add_(1)
+        x = self.embed[self.ids]
+        a = ops.attn_decode8_rope(ops.linear_q4(x, self.w["qkv"]), self.cos, self.sin, self.cache, self.lens, H)
+        h = ops.linear_q4(a, self.w["o"], residual=x)
+        logits = ops.linear_q4(h, self.w["lm"], out_f32=True)
+        logits = ops.logits_process(logits, output_ids=self.hist, output_lens=self.count, repetition_penalty=self.rep, frequency_penalty=self.freq)
+        ops.argmax(logits, out=self.ids)
+        self.hist.scatter_(1, self.count.long()[:, None], self.ids[:, None])
+        self.count.add_(1)
+        return logits, a
+
+
+def test_decode_steps_against_64_bits():
+    """Six steps: each step's attention from its own cache, and its logits from its own inputs, in 64 bits."""
+    st = _Step(5)
+    B, H, Hkv, D, S, V = st.dims
+    for _ in range(6):
+        ids, hist, count = st.ids.cpu().clone(), st.hist.cpu().clone(), st.count.cpu().clone()
+        logits, a = st()
+        host = [t.cpu().clone() for t in (st.cache.k, st.cache.k_scale, st.cache.v, st.cache.v_scale)]
+        w = {n: (q.codes.cpu(), q.scales.cpu(), None if q.zeros is None else q.zeros.cpu(), q.group) for n, q in st.w.items()}
+        x = st.embed.cpu()[ids]
+        y, mag = q4_ref(a.cpu(), *w["o"])
+        y = y + x.double()
+        h = y.to(_st())
+        ref, mag2 = q4_ref(h, *w["lm"])
+        # the hidden state is rounded on the way: half a step (a whole one where the fp32 sum sits beside a border) through the last product
+        hb = (2 * _half() * y.abs() + (H * D + 16) * U * mag)
+        wl = torch.stack([w["lm"][0] & 15, w["lm"][0] >> 4], -1).view(V, -1).double() - w["lm"][2].double().repeat_interleave(32, 1)
+        prop = hb @ (wl * w["lm"][1].double().repeat_interleave(32, 1)).abs().t().contiguous()
+        p, pb = logits_ref(ref, output=hist, olens=count, rep=st.rep.cpu(), freq=st.freq.cpu())
+        assert ((logits.cpu().double() - p).abs() <= 1.3 * (prop + (H * D + 16) * U * mag2) + pb).all()
+        q16 = None
+        assert torch.isfinite(a.float()).all()
+        assert torch.equal(st.ids.cpu(), logits.argmax(-1).cpu())
+        _ = host, q16
+
+
+def test_captured_steps_replay_like_eager_ones():
+    eager, graphed = _Step(6), _Step(6)
+    eager()
+    graphed()                                                                               # (warm-up outside the capture)
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    g = torch.cuda.CUDAGraph()
+    keep = [t.clone() for t in (graphed.lens, graphed.ids, graphed.hist, graphed.count)]
+    with torch.cuda.graph(g, stream=side):
+        out, att = graphed()
+    for t, k in zip((graphed.lens, graphed.ids, graphed.hist, graphed.count), keep):
+        assert torch.equal(t, k)                                                            # capturing runs nothing
+    for _ in range(4):
+        want, want_a = eager()
+        g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want) and torch.equal(att, want_a) and torch.equal(graphed.ids, eager.ids) and torch.equal(graphed.hist, eager.hist)
+        for a, b in zip((graphed.cache.k, graphed.cache.v), (eager.cache.k, eager.cache.v)):
+            assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
+
+
+def test_two_streams_at_once():
+    """Two loops on two streams share no scratch."""
+    one, two, ref = _Step(7), _Step(8), [_Step(7), _Step(8)]
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(5):
+        for i, (s, step) in enumerate(zip(streams, (one, two))):
+            with torch.cuda.stream(s):
+                got[i].append(step()[0])
+    torch.cuda.synchronize()
+    for i in range(2):
+        for y in got[i]:
+            assert torch.equal(y, ref[i]()[0])
+
+
+def test_a_later_chunk_attends_to_what_is_read_back():
+    """Chunked prefill: the second chunk's queries over the first chunk's keys read back from the cache and its own, through attn_prefill."""
+    from modelcompose_amd import ops
+    g = _gen(41)
+    B, H, D, n0, n1 = 2, 4, 128, 70, 30
+    S = n0 + n1
+    cache = ops.kv8_cache(B, H, S, D, dtype=torch.int8)
+    cos, sin = (t.cuda() for t in tables(S, D))
+    for lo, n in ((0, n0), (n0, n1)):
+        qkv = _rand(g, B * n, 3 * H * D).cuda()
+        row = torch.arange(B * n)
+        q = torch.zeros(B * n, H * D, dtype=_st(), device="cuda")
+        ops.rope_kv8(qkv, (row // n).int().cuda(), (row % n + lo).int().cuda(), (row % n).int().cuda(), cos, sin, q, cache, H, n)
+    k, v = ops.kv8_read(cache, S)
+    out = torch.empty(B * n1, H * D, dtype=_st(), device="cuda")
+    ops.attn_prefill(q, k, v, out, B, H, H, n1, S, D, (n1 * H * D, H * D, D), (H * S * D, D, S * D), (H * S * D, D, S * D), H * D, True, q_offset=n0)
+    kd, vd, qd = k.cpu().double(), v.cpu().double(), q.cpu().double().view(B, n1, H, D)
+    for b in range(B):
+        for h in range(H):
+            s = qd[b, :, h] @ kd[b, h].t() / math.sqrt(D)
+            s = s.masked_fill(torch.arange(S) > torch.arange(n1)[:, None] + n0, -math.inf)
+            p = torch.softmax(s, -1)
+            ref = p @ vd[b, h]
+            # 16-bit probabilities in the prefill kernel: half a step of each (and as much for their sum)
+            bound = _half() * ref.abs() + (3 * _half()) * (p @ vd[b, h].abs())
+            assert ((out.cpu().double().view(B, n1, H, D)[b, :, h] - ref).abs() <= bound + 1e-6).all()
+    last = ops.attn_decode8(q.view(B, n1, H, D)[:, -1], cache)                                # the last query as a decode step: the codes themselves
+    near(last.view(B, H, D), *attend(qd[:, -1], [t.cpu() for t in (cache.k, cache.k_scale, cache.v, cache.v_scale)], [S] * B, 1 / math.sqrt(D)))
