@@ -29,6 +29,11 @@ def _half():
     return torch.finfo(_st()).eps / 2
 
 
+def _stored(ref):
+    """What rounding ref to the storage dtype may add: half a step, which below the smallest normal number (fp16: 2^-14) is that of the subnormals."""
+    return _half() * ref.abs().clamp_min(torch.finfo(_st()).tiny)
+
+
 def _gen(seed):
     return torch.Generator().manual_seed(seed)
 
@@ -104,7 +109,7 @@ def attend(q, host, lens, scale, key_valid=None):
             # score: D fused or D separately rounded products of fp32, two scalings; the weights carry its absolute error as a relative one, doubled
             # by the normalisation; n terms are summed, and each weight is held to 2^-17 or better
             delta = (D + 4) * U * (k.abs() @ q[b, h].abs() * abs(scale)).max()
-            bound[b, h] = _half() * out[b, h].abs() + (2 * delta + (len(at) + 16) * 2 * U + 2.0 ** -16) * (p @ v.abs()) + 1e-30
+            bound[b, h] = _stored(out[b, h]) + (2 * delta + (len(at) + 16) * 2 * U + 2.0 ** -16) * (p @ v.abs()) + 1e-30
     return out, bound
 
 
@@ -407,7 +412,7 @@ def test_linear_q4(M, N, K, group, zeros):
     near(y32, ref, err + 1e-30)
     y = ops.linear_q4(x.cuda(), w, residual=res.cuda())
     full = ref + bias.double() + res.double()
-    near(y, full, _half() * full.abs() + err * 1.01 + 3 * U * (ref.abs() + bias.double().abs() + res.double().abs()) + 1e-30)
+    near(y, full, _stored(full) + err * 1.01 + 3 * U * (ref.abs() + bias.double().abs() + res.double().abs()) + 1e-30)
     # strided rows in and out, and a row's bits in another batch
     xs = torch.empty(M, K + 24, dtype=_st(), device="cuda")[:, :K]
     xs.copy_(x)
@@ -581,7 +586,7 @@ def test_decode_steps_against_64_bits():
         h = y.to(_st())
         ref, mag2 = q4_ref(h, *w["lm"])
         # the hidden state is rounded on the way: half a step (a whole one where the fp32 sum sits beside a border) through the last product
-        hb = (2 * _half() * y.abs() + (H * D + 16) * U * mag)
+        hb = (2 * _stored(y) + (H * D + 16) * U * mag)
         wl = torch.stack([w["lm"][0] & 15, w["lm"][0] >> 4], -1).view(V, -1).double() - w["lm"][2].double().repeat_interleave(32, 1)
         prop = hb @ (wl * w["lm"][1].double().repeat_interleave(32, 1)).abs().t().contiguous()
         p, pb = logits_ref(ref, output=hist, olens=count, rep=st.rep.cpu(), freq=st.freq.cpu())
@@ -654,7 +659,7 @@ def test_a_later_chunk_attends_to_what_is_read_back():
             p = torch.softmax(s, -1)
             ref = p @ vd[b, h]
             # 16-bit probabilities in the prefill kernel: half a step of each (and as much for their sum)
-            bound = _half() * ref.abs() + (3 * _half()) * (p @ vd[b, h].abs())
+            bound = _stored(ref) + (3 * _half()) * (p @ vd[b, h].abs())
             assert ((out.cpu().double().view(B, n1, H, D)[b, :, h] - ref).abs() <= bound + 1e-6).all()
     last = ops.attn_decode8(q.view(B, n1, H, D)[:, -1], cache)                                # the last query as a decode step: the codes themselves
     near(last.view(B, H, D), *attend(qd[:, -1], [t.cpu() for t in (cache.k, cache.k_scale, cache.v, cache.v_scale)], [S] * B, 1 / math.sqrt(D)))
