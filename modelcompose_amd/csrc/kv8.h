@@ -48,3 +48,51 @@ __device__ __forceinline__ void kv8_unpack4(uint32_t w, float (&f)[4]) {
         f[0] = (float)(int8_t)(w & 255); f[1] = (float)(int8_t)((w >> 8) & 255); f[2] = (float)(int8_t)((w >> 16) & 255); f[3] = (float)((int32_t)w >> 24);
     }
 }
+
+// ---- matrix-instruction operands from codes ------------------------------------------------------------------------------------------
+typedef __bf16 kv8_b16x2 __attribute__((ext_vector_type(2)));
+typedef __bf16 kv8_b16x8 __attribute__((ext_vector_type(8)));        // bfloat16 in both builds: the value operand (below)
+
+// Codes b0, b1 of half HI of a word as one word of two 16-bit floats; every code is exact in bfloat16 and in IEEE half.
+template <int FMT, bool F16, bool HI>
+__device__ __forceinline__ uint32_t kv8_pair(uint32_t w) {
+    if constexpr (FMT == MC_KV8_E4M3) {
+        if constexpr (F16) return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.0f, HI));
+        else return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, HI));
+    } else {
+        float a, b;                                                  // the byte is picked and sign-extended by the conversion itself
+        if constexpr (HI) {
+            asm("v_cvt_f32_i32_sdwa %0, sext(%1) dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:BYTE_2" : "=v"(a) : "v"(w));
+            asm("v_cvt_f32_i32_sdwa %0, sext(%1) dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:BYTE_3" : "=v"(b) : "v"(w));
+        } else {
+            asm("v_cvt_f32_i32_sdwa %0, sext(%1) dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:BYTE_0" : "=v"(a) : "v"(w));
+            asm("v_cvt_f32_i32_sdwa %0, sext(%1) dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:BYTE_1" : "=v"(b) : "v"(w));
+        }
+        if constexpr (F16) return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(a, b));
+        else return __builtin_amdgcn_perm(__float_as_uint(b), __float_as_uint(a), 0x07060302u);      // the high halves: integers below 2^8 end there
+    }
+}
+// the largest / the sum of a value over the lanes lane ^ 16, lane ^ 32, lane ^ 48, in every lane (row swaps instead of LDS shuffles)
+__device__ __forceinline__ float kv8_quarters_max(float x) {
+    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    x = fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+    const auto t = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return fmaxf(__uint_as_float(t[0]), __uint_as_float(t[1]));
+}
+__device__ __forceinline__ float kv8_quarters_sum(float x) {
+    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    x = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+    const auto t = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return __uint_as_float(t[0]) + __uint_as_float(t[1]);
+}
+// the value of lane ^ 8 (rotation by 8 within each row of 16)
+__device__ __forceinline__ float kv8_other_half(float x) {
+    return __uint_as_float((uint32_t)__builtin_amdgcn_update_dpp(0, (int)__float_as_uint(x), 0x128, 0xf, 0xf, true));
+}
+// eight consecutive codes as an operand of the storage element (keys against the queries)
+template <int FMT>
+__device__ __forceinline__ bf16x8 kv8_row8(uint32_t w0, uint32_t w1) {
+    constexpr bool F16 = MC_STORAGE_IS_F16;
+    const u32x4 o = {kv8_pair<FMT, F16, false>(w0), kv8_pair<FMT, F16, true>(w0), kv8_pair<FMT, F16, false>(w1), kv8_pair<FMT, F16, true>(w1)};
+    return __builtin_bit_cast(bf16x8, o);
+}

@@ -5,6 +5,8 @@
 // time reading them.
 #include "kv8.h"
 
+#include <type_traits>
+
 namespace {
 
 struct Cache {
@@ -16,8 +18,7 @@ struct Cache {
 // ---- cache write ------------------------------------------------------------------------------------------------------------------
 struct RopeParams {
     const bf16_t* qkv; int64_t ld;
-    const int32_t* row_b; const int32_t* row_pos; const int32_t* row_t;      // row_b null: row r is sequence r, position kv_lens[r] - 1, query row 0
-    const int32_t* kv_lens;
+    const int32_t* row_b; const int32_t* row_pos; const int32_t* row_t;
     const float* cosT; const float* sinT; int max_pos;
     bf16_t* q_out; Cache c;
     int M, H, Lq, blocks_per_row;
@@ -32,9 +33,7 @@ __global__ __launch_bounds__(256) void rope_kv8_kernel(RopeParams p) {
     const int row = blockIdx.x / p.blocks_per_row;
     const int vec = (blockIdx.x - row * p.blocks_per_row) * VPB + threadIdx.x / LPV, i4 = (threadIdx.x % LPV) * 4;
     if (vec >= p.H + 2 * p.c.Hkv) return;                       // (whole groups of LPV lanes leave: the shuffles below stay inside a group)
-    int b, pos, t;
-    if (p.row_b) { b = p.row_b[row]; pos = p.row_pos[row]; t = p.row_t[row]; }
-    else { b = row; pos = p.kv_lens[row] - 1; t = 0; }
+    const int b = p.row_b[row], pos = p.row_pos[row], t = p.row_t[row];
     // rows of no sequence (b < 0: padding), and rows that do not fit the cache, the tables or q_out: nothing is written
     if (b < 0 || b >= p.c.B || pos < 0 || pos >= p.c.S || pos >= p.max_pos || t < 0 || t >= p.Lq) return;
     const bf16_t* x = p.qkv + (int64_t)row * p.ld + (int64_t)vec * D + i4;
@@ -111,103 +110,386 @@ __global__ __launch_bounds__(256) void kv8_read_kernel(Cache c, const int32_t* k
 
 // ---- decode attention -------------------------------------------------------------------------------------------------------------
 struct AttnParams8 {
-    const bf16_t* q; int64_t q_sb, q_sh;
+    const bf16_t* q; int64_t q_sb, q_sh;           // query heads (rotated), or with `cosT` the pre-rotary rows q | k | v of the step's tokens (q_sb their stride)
     Cache c;
     bf16_t* o; int64_t o_sb;
+    float* ws;                                     // [B][H][ws_chunks][D + 4] partials: acc[D], m, l, -, -
     const int32_t* kv_lens; const uint8_t* key_valid; int64_t kv_stride;
-    int H, appended, max_pos;          // appended: the last key is this step's token; lengths that could not be appended give a zero row
+    const float* cosT; const float* sinT; int max_pos;
+    int H, G, groups, ws_chunks, self_combine;     // G = H / Hkv query heads per key head, in `groups` groups of at most 8
     float scale_log2e;
 };
 
+// number of keys; with an append, lengths that could not be appended count as none
 __device__ __forceinline__ int attn8_len(const AttnParams8& p, int b) {
     const int n = p.kv_lens ? p.kv_lens[b] : p.c.S;
-    if (p.appended && (n > p.c.S || n > p.max_pos)) return 0;
-    return min(n, p.c.S);
+    if (p.cosT && (n > p.c.S || n > p.max_pos)) return 0;
+    return max(0, min(n, p.c.S));
 }
 
-// One workgroup per query head; a key is held by D / 16 lanes; every group of lanes runs the online softmax over its keys.
-template <int D, int FMT>
-__global__ __launch_bounds__(256) void attn_decode8_kernel(AttnParams8 p) {
-    // a score and the maximum taken from it have to be the same number: fused into the difference, the score's product is not rounded, and at 1e30 what
-    // it differs by is no longer small
+// Keys of one partial: a function of the sequence's own length, so that short sequences still spread over many workgroups and long ones are not ground into
+// partials.
+__host__ __device__ inline int attn8_chunk(int n) { return n <= 4096 ? 512 : n <= 16384 ? 1024 : 2048; }
+typedef float f32x4_u __attribute__((ext_vector_type(4), aligned(4)));
+typedef uint32_t u32x2_u __attribute__((ext_vector_type(2), aligned(1)));
+
+// The partials (acc[D], m, l) of one head -> its output row, by a workgroup of 256.  In batches of up to 256: the batch's weights exp2(m - running maximum) are
+// computed by one thread each and kept in LDS; thread (s, d) adds the partials s, s + 256 / D, .. of element d; the 256 / D sums are added in order.
+template <int D>
+__device__ __forceinline__ void attn8_join(const float* parts, int np, bf16_t* o, float* lds) {
 #pragma clang fp contract(off)
-    constexpr int LPK = D / 16, KPW = 64 / LPK;
-    __shared__ float red[4][D + 2];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int b = blockIdx.x / p.H, h = blockIdx.x % p.H, hk = h / (p.H / p.c.Hkv);
-    const int n = attn8_len(p, b);
-    const int slot = lane / LPK, dl = (lane % LPK) * 16;
-    float q[16], acc[16], m = -1e30f, l = 0.f;
+    constexpr int SEG = 256 / D;
+    const int tid = threadIdx.x, d = tid % D, sg = tid / D;
+    float top = -INFINITY, ll = 0.f, aa = 0.f;         // ll: this thread's share of the sum
+    for (int c0 = 0; c0 < np; c0 += 256) {
+        const int cn = min(256, np - c0);
+        const float* batch = parts + (int64_t)c0 * (D + 4);
+        float m = -INFINITY, l = 0.f;
+        if (tid < cn) { m = batch[(int64_t)tid * (D + 4) + D]; l = batch[(int64_t)tid * (D + 4) + D + 1]; }
+        const float wm = wave_max(m);
+        __syncthreads();
+        if ((tid & 63) == 0) lds[256 + (tid >> 6)] = wm;
+        __syncthreads();
+        float mn = top;
 #pragma unroll
-    for (int i = 0; i < 16; ++i) { q[i] = n > 0 ? (float)p.q[b * p.q_sb + h * p.q_sh + dl + i] : 0.f; acc[i] = 0.f; }
-    const uint8_t* kb = p.c.k + b * p.c.sb + hk * p.c.sh + dl;
-    const uint8_t* vb = p.c.v + b * p.c.sb + hk * p.c.sh + dl;
-    for (int j0 = wave * KPW; j0 < n; j0 += 4 * KPW) {
-        const int j = j0 + slot;
-        const bool ok = j < n && (!p.key_valid || p.key_valid[b * p.kv_stride + j]);
-        u32x4 kw = {}, vw = {};
-        float ks = 0.f, vs = 0.f;
-        if (ok) {
-            kw = *(const u32x4*)(kb + j * p.c.st);
-            vw = *(const u32x4*)(vb + j * p.c.st);
-            ks = p.c.ks[b * p.c.ssb + hk * p.c.ssh + j];
-            vs = p.c.vs[b * p.c.ssb + hk * p.c.ssh + j];
+        for (int w = 0; w < 4; ++w) mn = fmaxf(mn, lds[256 + w]);
+        const float base = mn == -INFINITY ? 0.f : mn;      // nothing attended yet, or nothing but NaN
+        const float a = __builtin_amdgcn_exp2f(m - base), old = __builtin_amdgcn_exp2f(top - base);
+        top = mn;
+        lds[tid] = a;
+        ll = fmaf(l, a, ll * old);
+        aa *= old;
+        __syncthreads();
+        int c = sg;
+        for (; c + 7 * SEG < cn; c += 8 * SEG) {
+            float x[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) x[j] = batch[(int64_t)(c + j * SEG) * (D + 4) + d];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) aa = fmaf(x[j], lds[c + j * SEG], aa);
         }
-        float s = 0.f, f[4];
-#pragma unroll
-        for (int w = 0; w < 4; ++w) {
-            kv8_unpack4<FMT>(kw[w], f);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) s = fmaf(q[4 * w + i], f[i], s);
-        }
-#pragma unroll
-        for (int o = 1; o < LPK; o <<= 1) s += __shfl_xor(s, o, 64);
-        s *= ks * p.scale_log2e;
-        const float mn = ok ? fmaxf(m, s) : m, a = __builtin_amdgcn_exp2f(m - mn), e = ok ? __builtin_amdgcn_exp2f(s - mn) : 0.f;
-        m = mn;
-        l = fmaf(l, a, e);
-        const float ev = ok ? e * vs : 0.f;
-#pragma unroll
-        for (int w = 0; w < 4; ++w) {
-            kv8_unpack4<FMT>(vw[w], f);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) acc[4 * w + i] = fmaf(ev, f[i], acc[4 * w + i] * a);
-        }
+        for (; c < cn; c += SEG) aa = fmaf(batch[(int64_t)c * (D + 4) + d], lds[c], aa);
     }
-#pragma unroll
-    for (int o = LPK; o < 64; o <<= 1) {
-        const float m2 = __shfl_xor(m, o, 64), l2 = __shfl_xor(l, o, 64), mn = fmaxf(m, m2);
-        const float a1 = __builtin_amdgcn_exp2f(m - mn), a2 = __builtin_amdgcn_exp2f(m2 - mn);
-        l = l * a1 + l2 * a2;
-#pragma unroll
-        for (int i = 0; i < 16; ++i) acc[i] = acc[i] * a1 + __shfl_xor(acc[i], o, 64) * a2;
-        m = mn;
-    }
-    if (slot == 0) {
-#pragma unroll
-        for (int i = 0; i < 16; ++i) red[wave][dl + i] = acc[i];
-        if (dl == 0) { red[wave][D] = m; red[wave][D + 1] = l; }
-    }
+    ll = wave_sum(ll);
     __syncthreads();
-    const int d = threadIdx.x;
-    if (d >= D) return;
-    float mm = -1e30f, ll = 0.f, aa = 0.f;
-    for (int w = 0; w < 4; ++w) mm = fmaxf(mm, red[w][D]);
-    for (int w = 0; w < 4; ++w) {
-        const float a = __builtin_amdgcn_exp2f(red[w][D] - mm);
-        ll = fmaf(red[w][D + 1], a, ll);
-        aa = fmaf(red[w][d], a, aa);
+    if ((tid & 63) == 0) lds[256 + (tid >> 6)] = ll;
+    lds[tid] = aa;
+    __syncthreads();
+    if (!sg) {
+        ll = (lds[256] + lds[257]) + (lds[258] + lds[259]);
+#pragma unroll
+        for (int s = 1; s < SEG; ++s) aa += lds[s * D + d];
+        o[d] = (bf16_t)(ll == 0.f ? 0.f : aa / ll);
     }
-    p.o[b * p.o_sb + h * D + d] = (bf16_t)(ll == 0.f ? 0.f : aa / ll);
+    __syncthreads();                                       // (the next head's join reuses lds)
+}
+
+// the step's token: its key rotated and its key and value quantised to position pos by the first 2 D / 8 lanes of a wave (rope_kv8_kernel's arithmetic)
+template <int D, int FMT>
+__device__ __forceinline__ void attn8_append(const AttnParams8& p, int b, int hk, int pos, int lane) {
+#pragma clang fp contract(off)
+    constexpr int LPV = D / 8;
+    const bool is_v = lane >= LPV, on = lane < 2 * LPV;
+    const int i4 = (lane % LPV) * 4;
+    const bf16_t* x = p.q + (int64_t)b * p.q_sb + (int64_t)(p.H + hk + (is_v ? p.c.Hkv : 0)) * D + i4;
+    float a[4] = {}, bb[4] = {};
+    if (on) {
+        const bf16x4 xa = *(const bf16x4*)x, xb = *(const bf16x4*)(x + D / 2);
+        const f32x4 cs = *(const f32x4*)(p.cosT + (int64_t)pos * (D / 2) + i4), sn = *(const f32x4*)(p.sinT + (int64_t)pos * (D / 2) + i4);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            a[j] = (float)xa[j]; bb[j] = (float)xb[j];
+            if (!is_v) {
+                const float u = a[j] * cs[j], w = bb[j] * sn[j], y = bb[j] * cs[j], z = a[j] * sn[j];
+                a[j] = u - w;
+                bb[j] = y + z;
+            }
+        }
+    }
+    uint32_t m = 0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) m = max(m, max(__float_as_uint(a[j]) & 0x7fffffffu, __float_as_uint(bb[j]) & 0x7fffffffu));
+#pragma unroll
+    for (int o = LPV / 2; o > 0; o >>= 1) m = max(m, (uint32_t)__shfl_xor((int)m, o, 64));
+    if (!on) return;
+    const Kv8Scale s = kv8_scale<FMT>(m);
+    uint8_t* dst = (is_v ? p.c.v : p.c.k) + b * p.c.sb + hk * p.c.sh + pos * p.c.st + i4;
+    *(uint32_t*)dst = kv8_pack4<FMT>(a[0], a[1], a[2], a[3], s);
+    *(uint32_t*)(dst + D / 2) = kv8_pack4<FMT>(bb[0], bb[1], bb[2], bb[3], s);
+    if (i4 == 0) (is_v ? p.c.vs : p.c.ks)[b * p.c.ssb + hk * p.c.ssh + pos] = s.scale;
+}
+
+// Decode attention on the matrix cores, for up to 8 query heads that share a key head.
+//
+// S^T = K Q^T: the keys are the rows (A operand, codes widened to 16 bits, exact), the heads the columns.  Of the 16 columns, column c and column c + 8 are
+// the same head; with row r of half t standing for key 8 (r >> 2) + 4 t + (r & 3), lane (c, g) ends up with the scores of keys 8 g .. 8 g + 7 of head
+// c & 7 - exactly the layout in which the next product O^T = V^T P^T wants its B operand, so the probabilities never leave the lane.  They
+// enter that product as bfloat16, a high part in columns 0 .. 7 and the remainder in columns 8 .. 15 (w = p * v_scale = hi + lo to 2^-17): the second half of
+// the columns carries the accuracy that 8 significant bits lack, at no instruction.  (bfloat16 also in the half-precision build: w has a wide range.)
+// V^T's operand needs 8 keys of one element per lane: 8 loads of D / 16 bytes per lane (whole 128-byte rows per quarter wave), the bytes paired by v_perm.
+//
+// A workgroup of 4 waves takes chunks of 512 keys, blockIdx.y, + gridDim.y, ..; wave w the 32-key tiles w, w + 4, .. of a chunk, from a fresh (m, l, acc); the
+// waves are joined through LDS in wave order, the chunks by attn8_join in chunk order.  Which workgroup takes which chunk changes no bit.
+template <int D, int FMT, bool KM>
+__global__ __launch_bounds__(256, D == 128 ? 3 : 4) void attn_decode8_kernel(AttnParams8 p) {
+    // (a score and the maximum taken from it have to be the same number: fused into the difference, the score's product would not be rounded, and at 1e30 the
+    // two no longer cancel)
+#pragma clang fp contract(off)
+    constexpr int NU = D / 64, NT = D / 16;
+    __shared__ __attribute__((aligned(16))) float red[2][4][8][D + 4];          // two chunks' worth: one barrier per chunk
+    const int tid = threadIdx.x, lane = tid & 63, c = lane & 15, g = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int grp = blockIdx.x % p.groups, bk = blockIdx.x / p.groups, b = bk / p.c.Hkv, hk = bk % p.c.Hkv;
+    const int h0 = hk * p.G + grp * 8, nh = min(8, p.G - grp * 8);
+    const int n = attn8_len(p, b), chunk = attn8_chunk(n), nch = (n + chunk - 1) / chunk;
+    const uint8_t* kb = p.c.k + b * p.c.sb + hk * p.c.sh;
+    const uint8_t* vb = p.c.v + b * p.c.sb + hk * p.c.sh;
+    const float* ksb = p.c.ks + b * p.c.ssb + hk * p.c.ssh;
+    const float* vsb = p.c.vs + b * p.c.ssb + hk * p.c.ssh;
+
+    if (p.cosT && n > 0 && (nch - 1) % gridDim.y == blockIdx.y) {       // this workgroup reads the new key: it appends it first
+        if (wave == 0) attn8_append<D, FMT>(p, b, hk, n - 1, lane);
+        __syncthreads();
+    }
+
+    // A wave's 32-key tile.  Rows: half h of K, key 8 (c >> 2) + 4 h + (c & 3), codes 64 u + 16 g .. + 15; V, key 8 g + j, codes (D / 16) c ..; scales of keys
+    // 8 g .. + 7.  Addresses are a uniform base plus one 32-bit lane offset each (32 rows span less than 2^31 bytes: host check).
+    u32x4 kr[2][NU];
+    uint32_t vr[8][NU];
+    float ks[8], vs[8];
+    const uint32_t st = (uint32_t)p.c.st, koff = (uint32_t)(8 * (c >> 2) + (c & 3)) * st + 16 * g, voff = (uint32_t)(8 * g) * st + c * (D / 16), soff = 8 * g;
+    auto load_k = [&](int key0) {
+        const uint8_t* t = kb + (int64_t)key0 * p.c.st;
+        const float* z = ksb + key0;
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int u = 0; u < NU; ++u) kr[h][u] = __builtin_nontemporal_load((const u32x4*)(t + 4 * h * p.c.st + 64 * u + koff));
+        const f32x4 s0 = *(const f32x4_u*)(z + soff), s1 = *(const f32x4_u*)(z + 4 + soff);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) { ks[j] = s0[j]; ks[4 + j] = s1[j]; }
+    };
+    auto load_v = [&](int key0) {
+        const uint8_t* t = vb + (int64_t)key0 * p.c.st;
+        const float* z = vsb + key0;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const uint8_t* r = t + j * p.c.st + voff;
+            if constexpr (NU == 2) { const u32x2 w = __builtin_nontemporal_load((const u32x2*)r); vr[j][0] = w[0]; vr[j][1] = w[1]; }
+            else vr[j][0] = __builtin_nontemporal_load((const uint32_t*)r);
+        }
+        const f32x4 s0 = *(const f32x4_u*)(z + soff), s1 = *(const f32x4_u*)(z + 4 + soff);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) { vs[j] = s0[j]; vs[4 + j] = s1[j]; }
+    };
+    // the last, partial tile: rows behind the end are read as the last row (and not attended)
+    auto load_tail = [&](int key0) {
+        const int last = n - 1 - key0;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const int64_t r = key0 + min(8 * (c >> 2) + 4 * h + (c & 3), last);
+#pragma unroll
+            for (int u = 0; u < NU; ++u) kr[h][u] = *(const u32x4*)(kb + r * p.c.st + 64 * u + 16 * g);
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const int64_t r = key0 + min(8 * g + j, last);
+#pragma unroll
+            for (int u = 0; u < NU; ++u) vr[j][u] = *(const uint32_t*)(vb + r * p.c.st + c * (D / 16) + 4 * u);
+            ks[j] = ksb[r];
+            vs[j] = vsb[r];
+        }
+    };
+
+    int ch = blockIdx.y, key0 = ch * chunk + wave * 32;
+    if (key0 + 32 <= n) { load_k(key0); load_v(key0); }
+
+    // the queries, as B operands: column c is head c & 7, step 2 u + e holds elements 64 u + 16 g + 8 e .. + 7
+    bf16x8 qf[2 * NU];
+    {
+        const bf16_t* x = p.q + (int64_t)b * p.q_sb + (int64_t)(h0 + min(c & 7, nh - 1)) * (p.cosT ? D : p.q_sh);
+#pragma unroll
+        for (int t = 0; t < 2 * NU; ++t) {
+            const int d = 64 * (t >> 1) + 16 * g + 8 * (t & 1);
+            qf[t] = *(const bf16x8*)(x + d);
+            if (p.cosT && n > 0) {
+                const bool lo = d < D / 2;
+                const bf16x8 y = *(const bf16x8*)(x + (lo ? d + D / 2 : d - D / 2));
+                const float* cr = p.cosT + (int64_t)(n - 1) * (D / 2) + (lo ? d : d - D / 2);
+                const float* sr = p.sinT + (int64_t)(n - 1) * (D / 2) + (lo ? d : d - D / 2);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const float a = (float)qf[t][i], z = (float)y[i];
+                    float o1, o2;
+                    mc_rope_pair(lo ? a : z, lo ? z : a, cr[i], sr[i], o1, o2);
+                    qf[t][i] = (bf16_t)(lo ? o1 : o2);
+                }
+            }
+        }
+    }
+
+    float m, l;
+    f32x4 acc[NT];
+    int flip = 0;
+    // One tile: the scores from kr / ks, then the outputs from vr / vs.  next_k, next_v request the following tile's rows as soon as this one's are used.
+    // ok: which of this lane's 8 keys are attended (MASKED; else all).
+    auto tile = [&](auto masked, uint32_t ok, auto&& next_k, auto&& next_v) {
+        constexpr bool MASKED = decltype(masked)::value;
+        f32x4 s[2];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) s[h] = (f32x4){0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int u = 0; u < NU; ++u)
+#pragma unroll
+            for (int e = 0; e < 2; ++e)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) s[h] = mc_mfma_16x16x32(kv8_row8<FMT>(kr[h][u][2 * e], kr[h][u][2 * e + 1]), qf[2 * u + e], s[h]);
+        float sc[8], mx = -INFINITY;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            sc[j] = s[j >> 2][j & 3] * (ks[j] * p.scale_log2e);
+            if (MASKED && !((ok >> j) & 1u)) sc[j] = -INFINITY;
+            mx = fmaxf(mx, sc[j]);
+        }
+        next_k();
+        mx = kv8_quarters_max(mx);
+        if (__any(mx > m)) {
+            const float mn = fmaxf(m, mx), a = m == mn ? 1.f : __builtin_amdgcn_exp2f(m - mn);      // (m = -inf: 0)
+            m = mn;
+            l *= a;
+#pragma unroll
+            for (int i = 0; i < NT; ++i) acc[i] *= a;
+        }
+        const float base = m == -INFINITY ? 0.f : m;
+        kv8_b16x8 pf;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const float e = __builtin_amdgcn_exp2f(sc[j] - base);
+            l += e;
+            float w = e * vs[j];
+            if (MASKED && !((ok >> j) & 1u)) {                      // nothing of a masked key: not its scale, not its codes (either may be no number)
+                w = 0.f;
+#pragma unroll
+                for (int u = 0; u < NU; ++u) vr[j][u] = 0u;
+            }
+            const __bf16 hi = (__bf16)w;
+            pf[j] = c < 8 ? hi : (__bf16)(w - (float)hi);
+        }
+        // V^T operands: element (D / 16) c + i of keys 8 g .. 8 g + 7
+#pragma unroll
+        for (int u = 0; u < NU; ++u) {
+            uint32_t pr[4][2];
+#pragma unroll
+            for (int k2 = 0; k2 < 4; ++k2) {
+                pr[k2][0] = __builtin_amdgcn_perm(vr[2 * k2 + 1][u], vr[2 * k2][u], 0x05010400u);       // elements 0 and 1 of two keys
+                pr[k2][1] = __builtin_amdgcn_perm(vr[2 * k2 + 1][u], vr[2 * k2][u], 0x07030602u);       // 2 and 3
+            }
+            if (u == NU - 1) next_v();
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                u32x4 o;
+#pragma unroll
+                for (int k2 = 0; k2 < 4; ++k2) o[k2] = i & 1 ? kv8_pair<FMT, false, true>(pr[k2][i >> 1]) : kv8_pair<FMT, false, false>(pr[k2][i >> 1]);
+                acc[4 * u + i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(kv8_b16x8, o), pf, acc[4 * u + i], 0, 0, 0);
+            }
+        }
+    };
+
+    for (; ch < nch; ch += gridDim.y) {
+        m = -INFINITY; l = 0.f;
+#pragma unroll
+        for (int i = 0; i < NT; ++i) acc[i] = (f32x4){0.f, 0.f, 0.f, 0.f};
+        const int end = (ch + 1) * chunk;
+        const uint8_t* kv = p.key_valid + (int64_t)b * p.kv_stride;
+        for (; key0 < end && key0 + 32 <= n; key0 += 128) {
+            const int next = key0 + 128 < end ? key0 + 128 : (ch + (int)gridDim.y) * chunk + wave * 32;
+            uint32_t ok = 0;
+            if constexpr (KM) {
+                const u32x2 w = *(const u32x2_u*)(kv + key0 + soff);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) ok |= ((w[j >> 2] >> (8 * (j & 3))) & 255u) ? 1u << j : 0u;
+            }
+            tile(std::integral_constant<bool, KM>{}, ok, [&] { if (next + 32 <= n) load_k(next); }, [&] { if (next + 32 <= n) load_v(next); });
+        }
+        if (key0 < end && key0 < n) {
+            load_tail(key0);
+            uint32_t ok = 0;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const int key = key0 + 8 * g + j;
+                bool in = key < n;
+                if constexpr (KM) in = in && kv[min(key, n - 1)] != 0;
+                ok |= in ? 1u << j : 0u;
+            }
+            tile(std::true_type{}, ok, [] {}, [] {});
+        }
+        key0 = (ch + (int)gridDim.y) * chunk + wave * 32;
+
+        // this wave's partial: high and low columns together, then over the quarters for l.  acc[i][r] is element NT (4 g + r) + i of head c
+        l = kv8_quarters_sum(l);
+#pragma unroll
+        for (int i = 0; i < NT; ++i)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) acc[i][r] += kv8_other_half(acc[i][r]);
+        if (c < nh) {
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+#pragma unroll
+                for (int i = 0; i < NT; i += 4) *(f32x4*)&red[flip][wave][c][NT * (4 * g + r) + i] = (f32x4){acc[i][r], acc[i + 1][r], acc[i + 2][r], acc[i + 3][r]};
+            if (g == 0) { red[flip][wave][c][D] = m; red[flip][wave][c][D + 1] = l; }
+        }
+        __syncthreads();
+        for (int e = tid; e < nh * D; e += 256) {
+            const int h = e / D, d = e % D;
+            const float (*r)[8][D + 4] = red[flip];
+            float mm = -INFINITY;
+#pragma unroll
+            for (int w_ = 0; w_ < 4; ++w_) mm = fmaxf(mm, r[w_][h][D]);
+            const float base = mm == -INFINITY ? 0.f : mm;
+            float ll = 0.f, aa = 0.f;
+#pragma unroll
+            for (int w_ = 0; w_ < 4; ++w_) {
+                const float a = __builtin_amdgcn_exp2f(r[w_][h][D] - base);
+                ll = fmaf(r[w_][h][D + 1], a, ll);
+                aa = fmaf(r[w_][h][d], a, aa);
+            }
+            float* part = p.ws + ((int64_t)(b * p.H + h0 + h) * p.ws_chunks + ch) * (D + 4);
+            part[d] = aa;
+            if (d == 0) { part[D] = mm; part[D + 1] = ll; }
+        }
+        flip ^= 1;                                          // (a wave cannot write this half again before all have passed the next chunk's barrier)
+    }
+    if (!p.self_combine) return;
+    __syncthreads();
+    for (int h = h0; h < h0 + nh; ++h)
+        attn8_join<D>(p.ws + (int64_t)(b * p.H + h) * p.ws_chunks * (D + 4), nch, p.o + (int64_t)b * p.o_sb + h * D, &red[0][0][0][0]);
+}
+
+template <int D>
+__global__ __launch_bounds__(256) void attn_decode8_join_kernel(AttnParams8 p) {
+    __shared__ float lds[260];
+    const int b = blockIdx.x / p.H, h = blockIdx.x % p.H, n = attn8_len(p, b), chunk = attn8_chunk(n);
+    attn8_join<D>(p.ws + (int64_t)blockIdx.x * p.ws_chunks * (D + 4), (n + chunk - 1) / chunk, p.o + (int64_t)b * p.o_sb + h * D, lds);
+}
+
+// the most partials any length up to S has (a length just below a change of the chunk has more than those above it)
+int attn8_max_parts(int S) {
+    int most = 0;
+    for (int n : {S, S < 4096 ? S : 4096, S < 16384 ? S : 16384}) {
+        const int c = attn8_chunk(n), parts = (n + c - 1) / c;
+        most = parts > most ? parts : most;
+    }
+    return most;
 }
 
 int check_cache(const mc_kv8_cache* c, const char* who) {
     MC_CHECK_ARG(c && c->k && c->v && c->k_scale && c->v_scale, "%s: null cache pointer", who);
     MC_CHECK_ARG(c->format == MC_KV8_E4M3 || c->format == MC_KV8_INT8, "%s: cache format %d", who, c->format);
     MC_CHECK_ARG(c->D == 64 || c->D == 128, "%s: head_dim %d not supported (64 or 128)", who, c->D);
-    MC_CHECK_ARG(c->B > 0 && c->Hkv > 0 && c->S > 0, "%s: bad cache shape B=%d Hkv=%d S=%d", who, c->B, c->Hkv, c->S);
+    MC_CHECK_ARG(c->B > 0 && c->Hkv > 0 && c->S > 0 && c->S <= (1 << 30), "%s: bad cache shape B=%d Hkv=%d S=%d", who, c->B, c->Hkv, c->S);
     MC_CHECK_ARG((int64_t)c->B * c->Hkv < (1LL << 24), "%s: B * Hkv = %lld is too large", who, (long long)c->B * c->Hkv);
     MC_CHECK_ARG(((uintptr_t)c->k | (uintptr_t)c->v) % 16 == 0 && (c->sb | c->sh | c->st) % 16 == 0, "%s: the codes' rows must be 16-byte aligned", who);
+    MC_CHECK_ARG(c->st > 0 && c->st < (1LL << 26), "%s: %lld bytes from one position to the next", who, (long long)c->st);
     MC_CHECK_ARG(((uintptr_t)c->k_scale | (uintptr_t)c->v_scale) % 4 == 0, "%s: the scales must be 4-byte aligned", who);
     return 0;
 }
@@ -216,19 +498,23 @@ Cache dev_cache(const mc_kv8_cache* c) {
     return Cache{(uint8_t*)c->k, c->k_scale, (uint8_t*)c->v, c->v_scale, c->sb, c->sh, c->st, c->scale_sb, c->scale_sh, c->B, c->Hkv, c->S};
 }
 
+#define KV8_MASKED(D, F) attn_decode8_kernel<D, F, true>
+#define KV8_PLAIN(D, F) attn_decode8_kernel<D, F, false>
+#define KV8_ROPE(D, F) rope_kv8_kernel<D, F>
+#define KV8_READ(D, F) kv8_read_kernel<D, F>
 #define KV8_DISPATCH(c, KERNEL, grid, block, lds, s, ...)                                                          \
     do {                                                                                                           \
-        if ((c)->D == 128 && (c)->format == MC_KV8_E4M3) KERNEL<128, MC_KV8_E4M3><<<grid, block, lds, s>>>(__VA_ARGS__); \
-        else if ((c)->D == 128) KERNEL<128, MC_KV8_INT8><<<grid, block, lds, s>>>(__VA_ARGS__);                     \
-        else if ((c)->format == MC_KV8_E4M3) KERNEL<64, MC_KV8_E4M3><<<grid, block, lds, s>>>(__VA_ARGS__);         \
-        else KERNEL<64, MC_KV8_INT8><<<grid, block, lds, s>>>(__VA_ARGS__);                                         \
+        if ((c)->D == 128 && (c)->format == MC_KV8_E4M3) KERNEL(128, MC_KV8_E4M3)<<<grid, block, lds, s>>>(__VA_ARGS__); \
+        else if ((c)->D == 128) KERNEL(128, MC_KV8_INT8)<<<grid, block, lds, s>>>(__VA_ARGS__);                     \
+        else if ((c)->format == MC_KV8_E4M3) KERNEL(64, MC_KV8_E4M3)<<<grid, block, lds, s>>>(__VA_ARGS__);         \
+        else KERNEL(64, MC_KV8_INT8)<<<grid, block, lds, s>>>(__VA_ARGS__);                                         \
     } while (0)
 
 int rope_launch(const mc_kv8_cache* c, RopeParams& p, hipStream_t s, const char* who) {
     const int nv = p.H + 2 * c->Hkv, vpb = 256 / (c->D / 8);
     p.blocks_per_row = (nv + vpb - 1) / vpb;
     MC_CHECK_ARG((int64_t)p.M * p.blocks_per_row < (1LL << 23), "%s: too many rows (%d of %d heads) for one launch", who, p.M, nv);
-    KV8_DISPATCH(c, rope_kv8_kernel, p.M * p.blocks_per_row, 256, 0, s, p);
+    KV8_DISPATCH(c, KV8_ROPE, p.M * p.blocks_per_row, 256, 0, s, p);
     MC_CHECK_LAUNCH();
     return 0;
 }
@@ -243,11 +529,23 @@ int check_rope(const void* qkv, int64_t ld, const float* cos_table, const float*
     return 0;
 }
 
-int attn8_launch(const void* q, int64_t q_sb, int64_t q_sh, const mc_kv8_cache* c, const int32_t* kv_lens, const void* key_valid, int64_t kv_stride,
-                 void* o, int64_t o_sb, int H, int appended, int max_pos, float scale, hipStream_t s) {
-    AttnParams8 p{(const bf16_t*)q, q_sb, q_sh, dev_cache(c), (bf16_t*)o, o_sb, kv_lens, (const uint8_t*)key_valid, kv_stride, H, appended, max_pos,
-                  scale * 1.4426950408889634f};
-    KV8_DISPATCH(c, attn_decode8_kernel, c->B * H, 256, 0, s, p);
+// enough workgroups to fill the chip several times over, while there are chunks to hand out
+int attn8_launch(AttnParams8& p, const mc_kv8_cache* c, hipStream_t s, const char* who) {
+    const int chunks = attn8_max_parts(c->S);
+    p.G = p.H / c->Hkv;
+    p.groups = (p.G + 7) / 8;
+    p.ws_chunks = chunks;
+    const int64_t wgs = (int64_t)c->B * c->Hkv * p.groups;
+    MC_CHECK_ARG(wgs < (1LL << 23) && (int64_t)c->B * p.H < (1LL << 23), "%s: B * H = %lld is too large for one launch", who, (long long)c->B * p.H);
+    const int want = (int)((4096 + wgs - 1) / wgs), split = want < chunks ? want : chunks;
+    p.self_combine = split == 1;
+    const dim3 grid((unsigned)wgs, split);
+    if (p.key_valid) KV8_DISPATCH(c, KV8_MASKED, grid, 256, 0, s, p);
+    else KV8_DISPATCH(c, KV8_PLAIN, grid, 256, 0, s, p);
+    if (!p.self_combine) {
+        if (c->D == 128) attn_decode8_join_kernel<128><<<c->B * p.H, 256, 0, s>>>(p);
+        else attn_decode8_join_kernel<64><<<c->B * p.H, 256, 0, s>>>(p);
+    }
     MC_CHECK_LAUNCH();
     return 0;
 }
@@ -260,7 +558,7 @@ extern "C" int mc_rope_kv8(const void* qkv, int64_t ld, const int32_t* row_b, co
     MC_CHECK_ARG(row_b && row_pos && row_t && q_out && (uintptr_t)q_out % 16 == 0, "mc_rope_kv8: null or misaligned pointer");
     MC_CHECK_ARG(M >= 0 && Lq > 0, "mc_rope_kv8: bad shape M=%d Lq=%d", M, Lq);
     if (M == 0) return 0;
-    RopeParams p{(const bf16_t*)qkv, ld, row_b, row_pos, row_t, nullptr, cos_table, sin_table, max_pos, (bf16_t*)q_out, dev_cache(cache), M, H, Lq, 0};
+    RopeParams p{(const bf16_t*)qkv, ld, row_b, row_pos, row_t, cos_table, sin_table, max_pos, (bf16_t*)q_out, dev_cache(cache), M, H, Lq, 0};
     return rope_launch(cache, p, (hipStream_t)stream, "mc_rope_kv8");
 }
 
@@ -273,15 +571,14 @@ extern "C" int mc_kv8_read(const mc_kv8_cache* cache, const int32_t* kv_lens, in
     MC_CHECK_ARG(blocks < (1LL << 23), "mc_kv8_read: %d positions are too many for one launch", n);
     const int bh = cache->B * cache->Hkv;
     const dim3 grid((unsigned)blocks, bh < 4096 ? bh : 4096);
-    KV8_DISPATCH(cache, kv8_read_kernel, grid, 256, 0, (hipStream_t)stream, dev_cache(cache), kv_lens, n, (bf16_t*)k_out, (bf16_t*)v_out);
+    KV8_DISPATCH(cache, KV8_READ, grid, 256, 0, (hipStream_t)stream, dev_cache(cache), kv_lens, n, (bf16_t*)k_out, (bf16_t*)v_out);
     MC_CHECK_LAUNCH();
     return 0;
 }
 
 extern "C" int mc_attn_decode8_workspace_bytes(int B, int H, int D, int S, int64_t* bytes) {
-    (void)S;
-    MC_CHECK_ARG(bytes && B > 0 && H > 0 && D > 0, "mc_attn_decode8_workspace_bytes: bad arguments");
-    *bytes = (int64_t)B * H * D * 2;
+    MC_CHECK_ARG(bytes && B > 0 && H > 0 && D > 0 && S > 0, "mc_attn_decode8_workspace_bytes: bad arguments");
+    *bytes = (int64_t)B * H * attn8_max_parts(S) * (D + 4) * 4;
     return 0;
 }
 
@@ -291,7 +588,9 @@ extern "C" int mc_attn_decode8(const void* q, int64_t q_sb, int64_t q_sh, const 
     MC_CHECK_ARG(q && o && workspace, "mc_attn_decode8: null pointer");
     MC_CHECK_ARG(H > 0 && H % cache->Hkv == 0, "mc_attn_decode8: %d query heads over %d key heads", H, cache->Hkv);
     MC_CHECK_ARG((uintptr_t)q % 16 == 0 && (q_sb | q_sh) % 8 == 0, "mc_attn_decode8: query rows must be 16-byte aligned");
-    return attn8_launch(q, q_sb, q_sh, cache, kv_lens, key_valid, key_valid_stride, o, o_sb, H, 0, 0, scale, (hipStream_t)stream);
+    AttnParams8 p{(const bf16_t*)q, q_sb, q_sh, dev_cache(cache), (bf16_t*)o, o_sb, (float*)workspace, kv_lens, (const uint8_t*)key_valid, key_valid_stride,
+                  nullptr, nullptr, 0, H, 0, 0, 0, 0, scale * 1.4426950408889634f};
+    return attn8_launch(p, cache, (hipStream_t)stream, "mc_attn_decode8");
 }
 
 extern "C" int mc_attn_decode8_rope(const void* qkv, int64_t qkv_ld, const float* cos_table, const float* sin_table, int max_pos, const mc_kv8_cache* cache,
@@ -299,8 +598,7 @@ extern "C" int mc_attn_decode8_rope(const void* qkv, int64_t qkv_ld, const float
                                     float scale, void* stream) {
     if (int e = check_rope(qkv, qkv_ld, cos_table, sin_table, max_pos, H, cache, "mc_attn_decode8_rope")) return e;
     MC_CHECK_ARG(kv_lens && o && workspace, "mc_attn_decode8_rope: null pointer");
-    const int D = cache->D;
-    RopeParams p{(const bf16_t*)qkv, qkv_ld, nullptr, nullptr, nullptr, kv_lens, cos_table, sin_table, max_pos, (bf16_t*)workspace, dev_cache(cache), cache->B, H, 1, 0};
-    if (int e = rope_launch(cache, p, (hipStream_t)stream, "mc_attn_decode8_rope")) return e;
-    return attn8_launch(workspace, (int64_t)H * D, D, cache, kv_lens, key_valid, key_valid_stride, o, o_sb, H, 1, max_pos, scale, (hipStream_t)stream);
+    AttnParams8 p{(const bf16_t*)qkv, qkv_ld, cache->D, dev_cache(cache), (bf16_t*)o, o_sb, (float*)workspace, kv_lens, (const uint8_t*)key_valid, key_valid_stride,
+                  cos_table, sin_table, max_pos, H, 0, 0, 0, 0, scale * 1.4426950408889634f};
+    return attn8_launch(p, cache, (hipStream_t)stream, "mc_attn_decode8_rope");
 }
