@@ -252,19 +252,24 @@ __global__ __launch_bounds__(256, D == 128 ? 3 : 4) void attn_decode8_kernel(Att
         __syncthreads();
     }
 
-    // A wave's 32-key tile.  Rows: half h of K, key 8 (c >> 2) + 4 h + (c & 3), codes 64 u + 16 g .. + 15; V, key 8 g + j, codes (D / 16) c ..; scales of keys
-    // 8 g .. + 7.  Addresses are a uniform base plus one 32-bit lane offset each (32 rows span less than 2^31 bytes: host check).
+    // A wave's 32-key tile.  The operands want, in lane (c, g): of half h of K, key 8 (c >> 2) + 4 h + (c & 3), codes 64 u + 16 g .. + 15; of V, key 8 g + j, the
+    // D / 16 codes from vd on; the scales of keys 8 g .. + 7.  With D = 128 rows are whole 128-byte lines, and a load that takes half lines of twice the
+    // rows runs 8-10 % slower (48 x 2809 keys, the loads alone: 149 against 138 us): lane c reads 16-byte pieces of the rows c & 7 and (c & 7) + 8 of a half (V: of
+    // an even or an odd key), eight lanes to a row, and swaps with lane c ^ 8 what belongs there (settle()).
+    // Addresses are a uniform base plus one 32-bit lane offset each (32 rows span less than 2^31 bytes: host check).
     u32x4 kr[2][NU];
     uint32_t vr[8][NU];
     float ks[8], vs[8];
-    const uint32_t st = (uint32_t)p.c.st, koff = (uint32_t)(8 * (c >> 2) + (c & 3)) * st + 16 * g, voff = (uint32_t)(8 * g) * st + c * (D / 16), soff = 8 * g;
+    const uint32_t st = (uint32_t)p.c.st, soff = 8 * g, vd = D == 128 ? 16 * (c & 7) + 8 * (c >> 3) : 4 * c;
+    const uint32_t koff = D == 128 ? (uint32_t)(8 * ((c & 7) >> 2) + (c & 3)) * st + 64 * (c >> 3) + 16 * g : (uint32_t)(8 * (c >> 2) + (c & 3)) * st + 16 * g;
+    const uint32_t voff = D == 128 ? (uint32_t)(8 * g + (c >> 3)) * st + 16 * (c & 7) : (uint32_t)(8 * g) * st + vd;
     auto load_k = [&](int key0) {
         const uint8_t* t = kb + (int64_t)key0 * p.c.st;
         const float* z = ksb + key0;
 #pragma unroll
         for (int h = 0; h < 2; ++h)
 #pragma unroll
-            for (int u = 0; u < NU; ++u) kr[h][u] = __builtin_nontemporal_load((const u32x4*)(t + 4 * h * p.c.st + 64 * u + koff));
+            for (int u = 0; u < NU; ++u) kr[h][u] = __builtin_nontemporal_load((const u32x4*)(t + (4 * h + 16 * u) * p.c.st + koff));
         const f32x4 s0 = *(const f32x4_u*)(z + soff), s1 = *(const f32x4_u*)(z + 4 + soff);
 #pragma unroll
         for (int j = 0; j < 4; ++j) { ks[j] = s0[j]; ks[4 + j] = s1[j]; }
@@ -273,14 +278,34 @@ __global__ __launch_bounds__(256, D == 128 ? 3 : 4) void attn_decode8_kernel(Att
         const uint8_t* t = vb + (int64_t)key0 * p.c.st;
         const float* z = vsb + key0;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
+        for (int j = 0; j < 8; j += NU) {
             const uint8_t* r = t + j * p.c.st + voff;
-            if constexpr (NU == 2) { const u32x2 w = __builtin_nontemporal_load((const u32x2*)r); vr[j][0] = w[0]; vr[j][1] = w[1]; }
-            else vr[j][0] = __builtin_nontemporal_load((const uint32_t*)r);
+            if constexpr (NU == 2) {
+                const u32x4 w = __builtin_nontemporal_load((const u32x4*)r);
+                vr[j][0] = w[0]; vr[j][1] = w[1]; vr[j + 1][0] = w[2]; vr[j + 1][1] = w[3];
+            } else vr[j][0] = __builtin_nontemporal_load((const uint32_t*)r);
         }
         const f32x4 s0 = *(const f32x4_u*)(z + soff), s1 = *(const f32x4_u*)(z + 4 + soff);
 #pragma unroll
         for (int j = 0; j < 4; ++j) { vs[j] = s0[j]; vs[4 + j] = s1[j]; }
+    };
+    // what the loads brought to where the operands want it: a takes the other's b in the upper 8 columns, b the other's a in the lower 8
+    auto swap8 = [](uint32_t& a, uint32_t& b) {
+        const uint32_t x = (uint32_t)__builtin_amdgcn_update_dpp((int)a, (int)b, 0x128, 0xf, 0xc, false);
+        b = (uint32_t)__builtin_amdgcn_update_dpp((int)b, (int)a, 0x128, 0xf, 0x3, false);
+        a = x;
+    };
+    auto settle_k = [&] {
+        if constexpr (NU == 2)
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int w = 0; w < 4; ++w) { uint32_t a = kr[h][0][w], b_ = kr[h][1][w]; swap8(a, b_); kr[h][0][w] = a; kr[h][1][w] = b_; }
+    };
+    auto settle_v = [&] {
+        if constexpr (NU == 2)
+#pragma unroll
+            for (int j = 0; j < 8; j += 2) { swap8(vr[j][0], vr[j + 1][0]); swap8(vr[j][1], vr[j + 1][1]); }
     };
     // the last, partial tile: rows behind the end are read as the last row (and not attended)
     auto load_tail = [&](int key0) {
@@ -295,7 +320,7 @@ __global__ __launch_bounds__(256, D == 128 ? 3 : 4) void attn_decode8_kernel(Att
         for (int j = 0; j < 8; ++j) {
             const int64_t r = key0 + min(8 * g + j, last);
 #pragma unroll
-            for (int u = 0; u < NU; ++u) vr[j][u] = *(const uint32_t*)(vb + r * p.c.st + c * (D / 16) + 4 * u);
+            for (int u = 0; u < NU; ++u) vr[j][u] = *(const uint32_t*)(vb + r * p.c.st + vd + 4 * u);
             ks[j] = ksb[r];
             vs[j] = vsb[r];
         }
@@ -332,9 +357,10 @@ __global__ __launch_bounds__(256, D == 128 ? 3 : 4) void attn_decode8_kernel(Att
     f32x4 acc[NT];
     int flip = 0;
     // One tile: the scores from kr / ks, then the outputs from vr / vs.  next_k, next_v request the following tile's rows as soon as this one's are used.
-    // ok: which of this lane's 8 keys are attended (MASKED; else all).
-    auto tile = [&](auto masked, uint32_t ok, auto&& next_k, auto&& next_v) {
-        constexpr bool MASKED = decltype(masked)::value;
+    // ok: which of this lane's 8 keys are attended (MASKED; else all).  raw: the registers are as load_k / load_v left them.
+    auto tile = [&](auto masked, auto raw, uint32_t ok, auto&& next_k, auto&& next_v) {
+        constexpr bool MASKED = decltype(masked)::value, RAW = decltype(raw)::value;
+        if constexpr (RAW) settle_k();
         f32x4 s[2];
 #pragma unroll
         for (int h = 0; h < 2; ++h) s[h] = (f32x4){0.f, 0.f, 0.f, 0.f};
@@ -361,6 +387,7 @@ __global__ __launch_bounds__(256, D == 128 ? 3 : 4) void attn_decode8_kernel(Att
             for (int i = 0; i < NT; ++i) acc[i] *= a;
         }
         const float base = m == -INFINITY ? 0.f : m;
+        if constexpr (RAW) settle_v();
         kv8_b16x8 pf;
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
@@ -375,7 +402,7 @@ __global__ __launch_bounds__(256, D == 128 ? 3 : 4) void attn_decode8_kernel(Att
             const __bf16 hi = (__bf16)w;
             pf[j] = c < 8 ? hi : (__bf16)(w - (float)hi);
         }
-        // V^T operands: element (D / 16) c + i of keys 8 g .. 8 g + 7
+        // V^T operands: row c of product i is element vd + i, of keys 8 g .. 8 g + 7
 #pragma unroll
         for (int u = 0; u < NU; ++u) {
             uint32_t pr[4][2];
@@ -409,7 +436,7 @@ __global__ __launch_bounds__(256, D == 128 ? 3 : 4) void attn_decode8_kernel(Att
 #pragma unroll
                 for (int j = 0; j < 8; ++j) ok |= ((w[j >> 2] >> (8 * (j & 3))) & 255u) ? 1u << j : 0u;
             }
-            tile(std::integral_constant<bool, KM>{}, ok, [&] { if (next + 32 <= n) load_k(next); }, [&] { if (next + 32 <= n) load_v(next); });
+            tile(std::integral_constant<bool, KM>{}, std::true_type{}, ok, [&] { if (next + 32 <= n) load_k(next); }, [&] { if (next + 32 <= n) load_v(next); });
         }
         if (key0 < end && key0 < n) {
             load_tail(key0);
@@ -421,11 +448,11 @@ __global__ __launch_bounds__(256, D == 128 ? 3 : 4) void attn_decode8_kernel(Att
                 if constexpr (KM) in = in && kv[min(key, n - 1)] != 0;
                 ok |= in ? 1u << j : 0u;
             }
-            tile(std::true_type{}, ok, [] {}, [] {});
+            tile(std::true_type{}, std::false_type{}, ok, [] {}, [] {});
         }
         key0 = (ch + (int)gridDim.y) * chunk + wave * 32;
 
-        // this wave's partial: high and low columns together, then over the quarters for l.  acc[i][r] is element NT (4 g + r) + i of head c
+        // this wave's partial: high and low columns together, then over the quarters for l.  acc[i][r] is row 4 g + r of product i, head c
         l = kv8_quarters_sum(l);
 #pragma unroll
         for (int i = 0; i < NT; ++i)
@@ -435,7 +462,7 @@ __global__ __launch_bounds__(256, D == 128 ? 3 : 4) void attn_decode8_kernel(Att
 #pragma unroll
             for (int r = 0; r < 4; ++r)
 #pragma unroll
-                for (int i = 0; i < NT; i += 4) *(f32x4*)&red[flip][wave][c][NT * (4 * g + r) + i] = (f32x4){acc[i][r], acc[i + 1][r], acc[i + 2][r], acc[i + 3][r]};
+                for (int i = 0; i < NT; i += 4) *(f32x4*)&red[flip][wave][c][(D == 128 ? 64 * (g & 1) + 16 * r + 8 * (g >> 1) : 16 * g + 4 * r) + i] = (f32x4){acc[i][r], acc[i + 1][r], acc[i + 2][r], acc[i + 3][r]};
             if (g == 0) { red[flip][wave][c][D] = m; red[flip][wave][c][D + 1] = l; }
         }
         __syncthreads();
