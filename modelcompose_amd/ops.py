@@ -626,35 +626,43 @@ def attn_decode_rope(qkv, cos, sin, k_cache, v_cache, out, kv_lens, B, H, Hkv, S
 
 
 # ---- low-precision serving: 4-bit weights, the 8-bit KV cache, logits processing (csrc/gemm_q4.hip, csrc/kv8.hip, csrc/logits.hip) -------
-# These launch on the current stream of their tensors' device, whichever device is current.
-def _call(name, dev, *args):
-    fn = getattr(_lib.lib(), name)
-    if dev.index == torch.cuda.current_device():
-        rc = fn(*args, torch.cuda.current_stream().cuda_stream)
+# A decode step's launches last a few microseconds, so the wrappers are kept short: one test of everything a tensor has to be, and a look at what was wrong only
+# when it fails.  They launch on the current stream of their tensors' device, whichever device is current.
+_fns: dict = {}
+_F32, _I32, _I64, _U8 = torch.float32, torch.int32, torch.int64, torch.uint8
+
+
+def _call(name, index, *args):
+    L = _lib.lib()
+    fn = _fns.get((L, name))
+    if fn is None:
+        fn = _fns[(L, name)] = getattr(L, name)
+    if index == torch.cuda.current_device():
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
     else:
-        with torch.cuda.device(dev):
-            rc = fn(*args, torch.cuda.current_stream().cuda_stream)
+        with torch.cuda.device(index):
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
     if rc:
         _lib.check(rc, name)
 
 
-def _same_device(dev, **tensors):
-    for name, t in tensors.items():
-        if t is not None and t.device != dev:
-            raise ValueError(f"{name} is on {t.device}, expected {dev}")
+def _device(t, name):
+    """Index of a tensor's device."""
+    i = t.get_device()
+    if i < 0:
+        raise ValueError(f"{name} must be a device (HIP) tensor; this path has no CPU fallback")
+    return i
 
 
-def _arg(t, name, dev, dtype, shape=None, last=True):
-    """Checks of an optional tensor argument -> its address (0 for None).  shape entries of None are free; last: elements of the last dimension adjacent."""
-    if t is None:
-        return 0
-    if t.device != dev:
-        raise ValueError(f"{name} must be on {dev}, got {t.device}")
-    if t.dtype != dtype:
-        raise ValueError(f"{name} must be {dtype}, got {t.dtype}")
-    if shape is not None and (t.dim() != len(shape) or any(w is not None and g != w for g, w in zip(t.shape, shape))):
-        raise ValueError(f"{name} must have shape {shape}, got {tuple(t.shape)}")
-    if last and t.dim() and t.shape[-1] > 1 and t.stride(-1) != 1:
+def _arg(t, name, index, dtype, shape):
+    """Address of a tensor that has to be of this device, type and shape, with the elements of its last dimension adjacent."""
+    if t.get_device() != index or t.dtype != dtype or t.shape != shape or (t.stride(-1) != 1 and shape[-1] > 1):
+        if t.get_device() != index:
+            raise ValueError(f"{name} must be on device {index}, got {t.device}")
+        if t.dtype != dtype:
+            raise ValueError(f"{name} must be {dtype}, got {t.dtype}")
+        if t.shape != shape:
+            raise ValueError(f"{name} must have shape {tuple(shape)}, got {tuple(t.shape)}")
         raise ValueError(f"{name}: elements of the last dimension must be adjacent")
     return t.data_ptr()
 
@@ -663,24 +671,28 @@ class Q4Weight:
     """A linear weight in 4 bits: W[n, k] = scales[n, k // group] * (code[n, k] - zeros[n, k // group]).
     codes uint8 [N, K / 2] (two codes to a byte, even k in the low half), scales [N, K / group] in the storage dtype, zeros uint8 [N, K / group] or None (8);
     group = K // scales.shape[1]: 32, 64 or 128.  bias (storage dtype [N]) as in PackedWeight."""
-    __slots__ = ("codes", "scales", "zeros", "bias", "N", "K", "group", "_c")
+    __slots__ = ("codes", "scales", "zeros", "bias", "N", "K", "group", "index", "_c")
 
     def __init__(self, codes, scales, zeros=None, bias=None):
-        if not codes.is_cuda:
-            raise ValueError("codes must be a device (HIP) tensor; this path has no CPU fallback")
-        dev = codes.device
-        pc = _arg(codes, "codes", dev, torch.uint8, (None, None))
-        N, K = codes.shape[0], codes.shape[1] * 2
-        ps = _arg(scales, "scales", dev, BF16, (N, None))
+        index = _device(codes, "codes")
+        if codes.dim() != 2 or scales.dim() != 2:
+            raise ValueError("codes must be 2-D [N, K / 2] and scales 2-D [N, K / group]")
+        N, half = codes.shape
         G = scales.shape[1]
-        if G == 0 or K % G or K // G not in (32, 64, 128):
+        K = 2 * half
+        group = K // G if G else 0
+        if group not in (32, 64, 128) or group * G != K:
             raise ValueError(f"scales give groups of {K}/{G} columns: 32, 64 or 128 are supported")
-        pz = _arg(zeros, "zeros", dev, torch.uint8, (N, G))
-        _arg(bias, "bias", dev, BF16, (N,))
+        pc = _arg(codes, "codes", index, _U8, (N, half))
+        ps = _arg(scales, "scales", index, BF16, (N, G))
+        pz = 0 if zeros is None else _arg(zeros, "zeros", index, _U8, (N, G))
+        if bias is not None:
+            _arg(bias, "bias", index, BF16, (N,))
         # (a single row has no row stride: torch may report anything there)
-        ld = lambda t, w: t.stride(0) if t.shape[0] > 1 else ceil_to(w, 16)
-        self.codes, self.scales, self.zeros, self.bias, self.N, self.K, self.group = codes, scales, zeros, bias, N, K, K // G
-        self._c = _lib.Q4WeightC(pc, ld(codes, K // 2), ps, ld(scales, G), pz, 0 if zeros is None else ld(zeros, G), N, K, K // G)
+        one = N < 2
+        self.codes, self.scales, self.zeros, self.bias, self.N, self.K, self.group, self.index = codes, scales, zeros, bias, N, K, group, index
+        self._c = _lib.Q4WeightC(pc, half if one else codes.stride(0), ps, G if one else scales.stride(0), pz,
+                                 0 if zeros is None else G if one else zeros.stride(0), N, K, group)
 
     @property
     def nbytes(self):
@@ -690,23 +702,23 @@ class Q4Weight:
 def quantize_q4(w: torch.Tensor, group: int = 128, symmetric: bool = True, bias: Optional[torch.Tensor] = None) -> Q4Weight:
     """[N, K] storage dtype -> Q4Weight: symmetric - scale = amax / 7 around code 8; else scale = range / 15 with a zero point per group."""
     _req(w, BF16, "weight")
-    if w.dim() != 2 or group not in (32, 64, 128) or w.shape[1] == 0 or w.shape[1] % group:
+    if w.dim() != 2 or group not in (32, 64, 128) or w.shape[0] == 0 or w.shape[1] == 0 or w.shape[1] % group:
         raise ValueError(f"weight must be 2-D [N, K] with K a multiple of the group (32, 64 or 128), got {tuple(w.shape)} and {group}")
     if w.stride(1) != 1 or w.stride(0) % 8 or w.stride(0) < w.shape[1] or w.data_ptr() % 16:
         w = w.contiguous()
     N, K = w.shape
-    codes = torch.empty(N, K // 2, dtype=torch.uint8, device=w.device)
+    codes = torch.empty(N, K // 2, dtype=_U8, device=w.device)
     scales = torch.empty(N, K // group, dtype=BF16, device=w.device)
-    zeros = None if symmetric else torch.empty(N, K // group, dtype=torch.uint8, device=w.device)
-    _call("mc_quantize_q4_bf16", w.device, w.data_ptr(), w.stride(0) if N > 1 else K, codes.data_ptr(), scales.data_ptr(), 0 if zeros is None else zeros.data_ptr(),
-          N, K, group)
+    zeros = None if symmetric else torch.empty(N, K // group, dtype=_U8, device=w.device)
+    _call("mc_quantize_q4_bf16", w.get_device(), w.data_ptr(), w.stride(0) if N > 1 else K, codes.data_ptr(), scales.data_ptr(),
+          0 if zeros is None else zeros.data_ptr(), N, K, group)
     return Q4Weight(codes, scales, zeros, bias)
 
 
 def dequantize_q4(w: Q4Weight) -> PackedWeight:
     """The 16-bit PackedWeight of a 4-bit weight (each element rounded once): linear() with more than 64 rows."""
     out = torch.empty(packed_elems(w.N, w.K), dtype=BF16, device=w.codes.device)
-    _call("mc_dequantize_q4_bf16", out.device, C.byref(w._c), out.data_ptr())
+    _call("mc_dequantize_q4_bf16", w.index, C.byref(w._c), out.data_ptr())
     return PackedWeight(out, w.N, w.K, w.bias)
 
 
@@ -714,50 +726,51 @@ def linear_q4(x: torch.Tensor, w: Q4Weight, residual: Optional[torch.Tensor] = N
               bias: bool = True) -> torch.Tensor:
     """out[M, N] = x W^T (+ bias) (+ residual) for at most 64 rows x [M, K] (the decode step's form of linear(); larger launches: linear(x,
     dequantize_q4(w)), with x padded to its Kp).  fp32 sums; the codes enter as exact integers.  A row's bits do not depend on M."""
-    if not x.is_cuda:
-        raise ValueError("x must be a device (HIP) tensor; this path has no CPU fallback")
-    dev = x.device
-    px = _arg(x, "x", dev, BF16, (None, w.K))
-    M, N = x.shape[0], w.N
+    index = _device(x, "x")
+    if x.dim() != 2:
+        raise ValueError("x must be 2-D [M, K]")
+    M, N, dt = x.shape[0], w.N, _F32 if out_f32 else BF16
+    px = _arg(x, "x", index, BF16, (M, w.K))
     if M > 64:
         raise ValueError(f"linear_q4 takes at most 64 rows, got {M}: use linear(x, dequantize_q4(w))")
-    _same_device(dev, codes=w.codes)
+    if w.index != index:
+        raise ValueError(f"the weight is on device {w.index}, x on device {index}")
     if out is None:
-        out = torch.empty(M, N, dtype=torch.float32 if out_f32 else BF16, device=dev)
-    po = _arg(out, "out", dev, torch.float32 if out_f32 else BF16, (M, N))
-    pr = _arg(residual, "residual", dev, BF16, (M, N))
-    b = w.bias if bias else None
-    if M == 0:
-        return out
-    _call("mc_linear_q4_bf16", dev, px, x.stride(0) if M > 1 else w.K, C.byref(w._c), 0 if b is None else b.data_ptr(), pr,
-          0 if residual is None else residual.stride(0), po, out.stride(0), M, 1 if out_f32 else 0)
+        out = torch.empty((M, N), dtype=dt, device=x.device)
+        po, ldo = out.data_ptr(), N
+    else:
+        po, ldo = _arg(out, "out", index, dt, (M, N)), out.stride(0)
+    pr, ldr = (0, 0) if residual is None else (_arg(residual, "residual", index, BF16, (M, N)), residual.stride(0))
+    if M:
+        _call("mc_linear_q4_bf16", index, px, x.stride(0) if M > 1 else w.K, w._c, w.bias.data_ptr() if bias and w.bias is not None else 0, pr, ldr, po, ldo, M,
+              1 if out_f32 else 0)
     return out
 
 
 class Kv8Cache:
     """An 8-bit KV cache of one layer: codes k, v [B, Hkv, S, D] (torch.float8_e4m3fn or torch.int8, equal strides, head_dim contiguous) and their fp32
     scales k_scale, v_scale [B, Hkv, S], one per vector.  kv8_cache() makes one; slices over the batch of an existing one are caches too."""
-    __slots__ = ("k", "k_scale", "v", "v_scale", "B", "Hkv", "S", "D", "_c")
+    __slots__ = ("k", "k_scale", "v", "v_scale", "B", "Hkv", "S", "D", "index", "_c")
+    _formats = {torch.float8_e4m3fn: 1, torch.int8: 2}
 
     def __init__(self, k, k_scale, v, v_scale):
-        if not k.is_cuda:
-            raise ValueError("the cache must be device (HIP) tensors; this path has no CPU fallback")
-        dev = k.device
-        if k.dtype not in (torch.float8_e4m3fn, torch.int8):
-            raise ValueError(f"codes must be float8_e4m3fn or int8, got {k.dtype}")
-        pk = _arg(k, "k", dev, k.dtype, (None, None, None, None))
-        pv = _arg(v, "v", dev, k.dtype, k.shape)
-        B, Hkv, S, D = k.shape
-        pks, pvs = _arg(k_scale, "k_scale", dev, torch.float32, (B, Hkv, S)), _arg(v_scale, "v_scale", dev, torch.float32, (B, Hkv, S))
-        if k.stride() != v.stride() or k_scale.stride() != v_scale.stride():
+        index = _device(k, "the cache")
+        fmt = self._formats.get(k.dtype)
+        if fmt is None or k.dim() != 4:
+            raise ValueError(f"codes must be float8_e4m3fn or int8 [B, Hkv, S, D], got {k.dtype} {tuple(k.shape)}")
+        B, Hkv, S, D = shape = k.shape
+        pk, pv = _arg(k, "k", index, k.dtype, shape), _arg(v, "v", index, k.dtype, shape)
+        pks, pvs = _arg(k_scale, "k_scale", index, _F32, shape[:3]), _arg(v_scale, "v_scale", index, _F32, shape[:3])
+        st, ss = k.stride(), k_scale.stride()
+        if st != v.stride() or ss != v_scale.stride():
             raise ValueError("k and v (and their scales) must have the same strides")
-        for t, dims in ((k, 3), (k_scale, 2)):
-            if any(t.shape[i] > 1 and t.stride(i) <= 0 for i in range(dims)):
-                raise ValueError("a cache has no broadcast dimensions")
-        st = [k.stride(i) if k.shape[i] > 1 else D for i in range(3)]
-        ss = [k_scale.stride(i) if k_scale.shape[i] > 1 else 1 for i in range(2)]
-        self.k, self.k_scale, self.v, self.v_scale, self.B, self.Hkv, self.S, self.D = k, k_scale, v, v_scale, B, Hkv, S, D
-        self._c = _lib.Kv8CacheC(pk, pks, pv, pvs, *(st[0], st[1], st[2]), ss[0], ss[1], B, Hkv, S, D, 1 if k.dtype == torch.float8_e4m3fn else 2)
+        # (a dimension of size 1 has no stride: torch may report anything there)
+        sb, sh, sp = st[0] if B > 1 else D, st[1] if Hkv > 1 else D, st[2] if S > 1 else D
+        zb, zh = ss[0] if B > 1 else 1, ss[1] if Hkv > 1 else 1
+        if not (sb > 0 and sh > 0 and sp > 0 and zb > 0 and zh > 0):
+            raise ValueError("a cache has no broadcast dimensions")
+        self.k, self.k_scale, self.v, self.v_scale, self.B, self.Hkv, self.S, self.D, self.index = k, k_scale, v, v_scale, B, Hkv, S, D, index
+        self._c = _lib.Kv8CacheC(pk, pks, pv, pvs, sb, sh, sp, zb, zh, B, Hkv, S, D, fmt)
 
     @property
     def nbytes(self):
@@ -767,35 +780,34 @@ class Kv8Cache:
 def kv8_cache(B, Hkv, S, D, device="cuda", dtype=torch.float8_e4m3fn) -> Kv8Cache:
     """An empty (all zero) cache of S positions."""
     z = lambda dt, *s: torch.zeros(s, dtype=dt, device=device)
-    k, v = (z(torch.uint8, B, Hkv, S, D).view(dtype) for _ in range(2))
-    return Kv8Cache(k, z(torch.float32, B, Hkv, S), v, z(torch.float32, B, Hkv, S))
+    k, v = (z(_U8, B, Hkv, S, D).view(dtype) for _ in range(2))
+    return Kv8Cache(k, z(_F32, B, Hkv, S), v, z(_F32, B, Hkv, S))
 
 
 def _rope_args(qkv, cos, sin, cache, H, rows):
-    dev = qkv.device
-    if not qkv.is_cuda:
-        raise ValueError("qkv must be a device (HIP) tensor; this path has no CPU fallback")
-    p = _arg(qkv, "qkv", dev, BF16, (rows, (H + 2 * cache.Hkv) * cache.D))
-    _same_device(dev, cache=cache.k)
-    pc = _arg(cos, "cos", dev, torch.float32, (None, cache.D // 2))
-    ps = _arg(sin, "sin", dev, torch.float32, cos.shape)
+    index, width = _device(qkv, "qkv"), (H + 2 * cache.Hkv) * cache.D
+    p = _arg(qkv, "qkv", index, BF16, (rows, width))
+    if cache.index != index:
+        raise ValueError(f"the cache is on device {cache.index}, qkv on device {index}")
+    n_pos = cos.shape[0]
+    pc, ps = _arg(cos, "cos", index, _F32, (n_pos, cache.D // 2)), _arg(sin, "sin", index, _F32, (n_pos, cache.D // 2))
     if not (cos.is_contiguous() and sin.is_contiguous()):
         raise ValueError("cos and sin must be contiguous")
-    return dev, p, qkv.stride(0) if qkv.shape[0] > 1 else qkv.shape[1], pc, ps, cos.shape[0]
+    return index, p, qkv.stride(0) if rows > 1 else width, pc, ps, n_pos
 
 
 def rope_kv8(qkv, row_b, row_pos, row_t, cos, sin, q_out, cache: Kv8Cache, H, Lq):
     """rope_kv() for an 8-bit cache: rows [M, (H + 2 Hkv) D] of a q|k|v projection -> rotated queries in q_out [B * Lq, H * D] (row row_b * Lq + row_t), rotated keys and the
     values quantised to position row_pos of sequence row_b.  Rows with row_b < 0, or outside the cache, the tables or q_out, are skipped; a position is
     written by at most one row of a call."""
-    dev, p, ld, pc, ps, n_pos = _rope_args(qkv, cos, sin, cache, H, None)
     M = qkv.shape[0]
-    rb, rp, rt = (_arg(t, n, dev, torch.int32, (M,)) for t, n in ((row_b, "row_b"), (row_pos, "row_pos"), (row_t, "row_t")))
-    pq = _arg(q_out, "q_out", dev, BF16)
+    index, p, ld, pc, ps, n_pos = _rope_args(qkv, cos, sin, cache, H, M)
+    rb, rp, rt = _arg(row_b, "row_b", index, _I32, (M,)), _arg(row_pos, "row_pos", index, _I32, (M,)), _arg(row_t, "row_t", index, _I32, (M,))
+    pq = _arg(q_out, "q_out", index, BF16, q_out.shape)
     if not q_out.is_contiguous() or q_out.numel() != cache.B * Lq * H * cache.D:
         raise ValueError(f"q_out must hold {cache.B} x {Lq} contiguous rows of {H * cache.D}")
     if M:
-        _call("mc_rope_kv8", dev, p, ld, rb, rp, rt, pc, ps, n_pos, pq, C.byref(cache._c), M, H, Lq)
+        _call("mc_rope_kv8", index, p, ld, rb, rp, rt, pc, ps, n_pos, pq, cache._c, M, H, Lq)
     return q_out
 
 
@@ -803,59 +815,71 @@ def kv8_read(cache: Kv8Cache, n=None, kv_lens=None):
     """The first n (default: all) positions in the storage dtype: (k, v) [B, Hkv, n, D]; positions from kv_lens[b] on are zeros.  What attn_prefill reads when a
     later chunk of a prompt attends to keys that are in the cache already."""
     n = cache.S if n is None else int(n)
-    dev = cache.k.device
-    pl = _arg(kv_lens, "kv_lens", dev, torch.int32, (cache.B,))
+    pl = 0 if kv_lens is None else _arg(kv_lens, "kv_lens", cache.index, _I32, (cache.B,))
     if n < 0 or n > cache.S:
         raise ValueError(f"{n} positions of a cache of {cache.S}")
-    k = torch.empty(cache.B, cache.Hkv, n, cache.D, dtype=BF16, device=dev)
+    k = torch.empty((cache.B, cache.Hkv, n, cache.D), dtype=BF16, device=cache.k.device)
     v = torch.empty_like(k)
     if n:
-        _call("mc_kv8_read", dev, C.byref(cache._c), pl, n, k.data_ptr(), v.data_ptr())
+        _call("mc_kv8_read", cache.index, cache._c, pl, n, k.data_ptr(), v.data_ptr())
     return k, v
 
 
-def _decode8_buffers(cache, H, out, key_valid, dev):
-    B, D = cache.B, cache.D
+_decode8_ws: dict = {}          # (B, H, D, S) -> bytes of scratch
+
+
+def _decode8_scratch(B, H, D, S):
+    n = C.c_int64(0)
+    _lib.check(_lib.lib().mc_attn_decode8_workspace_bytes(B, H, D, S, C.byref(n)), "mc_attn_decode8_workspace_bytes")
+    if len(_decode8_ws) >= 4096:
+        _decode8_ws.clear()
+    _decode8_ws[(B, H, D, S)] = n.value
+    return n.value
+
+
+def _decode8(name, head, cache, H, kv_lens, out, scale, key_valid):
+    """The arguments that attn_decode8 and attn_decode8_rope share, and the call.  The scratch is the caching allocator's: calls in flight on other streams, and
+    captured graphs, have their own."""
+    B, D, S, index = cache.B, cache.D, cache.S, cache.index
+    dev = cache.k.device
+    pl = 0 if kv_lens is None else _arg(kv_lens, "kv_lens", index, _I32, (B,))
+    pm = ms = 0
+    if key_valid is not None:
+        if key_valid.dtype == torch.bool:
+            key_valid = key_valid.view(_U8)
+        if key_valid.dim() != 2 or key_valid.shape[1] < S:
+            raise ValueError(f"key_valid must be [B, >= {S}], got {tuple(key_valid.shape)}")
+        pm, ms = _arg(key_valid, "key_valid", index, _U8, (B, key_valid.shape[1])), key_valid.stride(0)
     if out is None:
-        out = torch.empty(B, H * D, dtype=BF16, device=dev)
-    po = _arg(out, "out", dev, BF16, (B, H * D))
-    if key_valid is not None and key_valid.dtype == torch.bool:
-        key_valid = key_valid.view(torch.uint8)
-    pm = _arg(key_valid, "key_valid", dev, torch.uint8, (B, None))
-    if key_valid is not None and key_valid.shape[1] < cache.S:
-        raise ValueError(f"key_valid covers {key_valid.shape[1]} positions, the cache has {cache.S}")
-    need = C.c_int64(0)
-    _lib.check(_lib.lib().mc_attn_decode8_workspace_bytes(B, H, D, cache.S, C.byref(need)), "mc_attn_decode8_workspace_bytes")
-    return out, po, pm, 0 if key_valid is None else key_valid.stride(0), torch.empty(need.value, dtype=torch.uint8, device=dev)
+        out = torch.empty((B, H * D), dtype=BF16, device=dev)
+        po, so = out.data_ptr(), H * D
+    else:
+        po, so = _arg(out, "out", index, BF16, (B, H * D)), out.stride(0)
+    ws = torch.empty(_decode8_ws.get((B, H, D, S)) or _decode8_scratch(B, H, D, S), dtype=_U8, device=dev)
+    _call(name, index, *head, cache._c, pl, pm, ms, po, so, ws.data_ptr(), H, D ** -0.5 if scale is None else scale)
+    return out
 
 
 def attn_decode8(q, cache: Kv8Cache, kv_lens=None, out=None, scale=None, key_valid=None):
     """Decode attention over an 8-bit cache: q [B, H, D] (one rotated query per sequence; H a multiple of Hkv), kv_lens int32 [B] (None: every position) ->
     out [B, H * D].  key_valid uint8 / bool [B, >= S]: 0 = masked.  A sequence without a key gives zeros."""
-    dev = q.device
-    if not q.is_cuda:
-        raise ValueError("q must be a device (HIP) tensor; this path has no CPU fallback")
-    pq = _arg(q, "q", dev, BF16, (cache.B, None, cache.D))
-    _same_device(dev, cache=cache.k)
+    index = _device(q, "q")
+    if q.dim() != 3:
+        raise ValueError("q must be [B, H, D]")
     H = q.shape[1]
-    pl = _arg(kv_lens, "kv_lens", dev, torch.int32, (cache.B,))
-    out, po, pm, ms, ws = _decode8_buffers(cache, H, out, key_valid, dev)
-    _call("mc_attn_decode8", dev, pq, q.stride(0), q.stride(1), C.byref(cache._c), pl, pm, ms, po, out.stride(0), ws.data_ptr(), H,
-          (1.0 / math.sqrt(cache.D)) if scale is None else scale)
-    return out
+    pq = _arg(q, "q", index, BF16, (cache.B, H, cache.D))
+    if cache.index != index:
+        raise ValueError(f"the cache is on device {cache.index}, q on device {index}")
+    return _decode8("mc_attn_decode8", (pq, q.stride(0) if cache.B > 1 else cache.D, q.stride(1) if H > 1 else cache.D), cache, H, kv_lens, out, scale, key_valid)
 
 
 def attn_decode8_rope(qkv, cos, sin, cache: Kv8Cache, kv_lens, H, out=None, scale=None, key_valid=None):
     """attn_decode_rope() over an 8-bit cache: the pre-rotary rows qkv [B, (H + 2 Hkv) D] of the tokens at positions kv_lens[b] - 1 (kv_lens int32 [B] counts them)
     are rotated, appended to the cache and attended.  A sequence with kv_lens[b] outside 1 .. min(S, rows of cos) is left alone: zeros, nothing written."""
-    dev, p, ld, pc, ps, n_pos = _rope_args(qkv, cos, sin, cache, H, cache.B)
-    pl = _arg(kv_lens, "kv_lens", dev, torch.int32, (cache.B,))
     if kv_lens is None:
         raise ValueError("kv_lens is needed: it places the new token")
-    out, po, pm, ms, ws = _decode8_buffers(cache, H, out, key_valid, dev)
-    _call("mc_attn_decode8_rope", dev, p, ld, pc, ps, n_pos, C.byref(cache._c), pl, pm, ms, po, out.stride(0), ws.data_ptr(), H,
-          (1.0 / math.sqrt(cache.D)) if scale is None else scale)
-    return out
+    index, p, ld, pc, ps, n_pos = _rope_args(qkv, cos, sin, cache, H, cache.B)
+    return _decode8("mc_attn_decode8_rope", (p, ld, pc, ps, n_pos), cache, H, kv_lens, out, scale, key_valid)
 
 
 def logits_process(logits, prompt_ids=None, prompt_lens=None, output_ids=None, output_lens=None, repetition_penalty=None, presence_penalty=None,
@@ -864,33 +888,41 @@ def logits_process(logits, prompt_ids=None, prompt_lens=None, output_ids=None, o
     prompt_ids / output_ids int64 [M, n] with optional int32 lengths [M]: the repetition penalty (l / r or l * r) reads both, frequency * count + presence
     only the output ids.  The penalties are fp32 tensors [M]; bias_ids int32 [M, n] with bias fp32 [M, n] (a token may be listed twice: the biases add up);
     allowed int32 [M, ceil(V / 32)]: bit t & 31 of word t >> 5 clear = -inf.  Ids outside [0, V) are ignored."""
-    if not logits.is_cuda:
-        raise ValueError("logits must be a device (HIP) tensor; this path has no CPU fallback")
-    dev, f32 = logits.device, torch.float32
-    pl = _arg(logits, "logits", dev, f32, (None, None))
+    index = _device(logits, "logits")
+    if logits.dim() != 2:
+        raise ValueError("logits must be 2-D [M, V]")
     M, V = logits.shape
+    pl = _arg(logits, "logits", index, _F32, (M, V))
     if out is None:
-        out = torch.empty(M, V, dtype=f32, device=dev)
-    a = _lib.LogitsArgsC(logits=pl, ld=logits.stride(0), out=_arg(out, "out", dev, f32, (M, V)), ld_out=out.stride(0), M=M, V=V)
-    if prompt_lens is not None and prompt_ids is None or output_lens is not None and output_ids is None:
-        raise ValueError("lengths without ids")
-    if prompt_ids is not None:
-        a.prompt_ids, a.ld_prompt, a.prompt_cols = _arg(prompt_ids, "prompt_ids", dev, torch.int64, (M, None)), prompt_ids.stride(0), prompt_ids.shape[1]
-        a.prompt_lens = _arg(prompt_lens, "prompt_lens", dev, torch.int32, (M,))
-    if output_ids is not None:
-        a.output_ids, a.ld_output, a.output_cols = _arg(output_ids, "output_ids", dev, torch.int64, (M, None)), output_ids.stride(0), output_ids.shape[1]
-        a.output_lens = _arg(output_lens, "output_lens", dev, torch.int32, (M,))
-    a.repetition, a.presence, a.frequency = (_arg(t, n, dev, f32, (M,)) for t, n in (
-        (repetition_penalty, "repetition_penalty"), (presence_penalty, "presence_penalty"), (frequency_penalty, "frequency_penalty")))
+        out = torch.empty((M, V), dtype=_F32, device=logits.device)
+        po, ldo = out.data_ptr(), V
+    else:
+        po, ldo = _arg(out, "out", index, _F32, (M, V)), out.stride(0)
+    hist = []
+    for name, ids, lens in (("prompt", prompt_ids, prompt_lens), ("output", output_ids, output_lens)):
+        if ids is None:
+            if lens is not None:
+                raise ValueError(f"{name}_lens without {name}_ids")
+            hist += (0, 0, 0, 0)
+            continue
+        if ids.dim() != 2:
+            raise ValueError(f"{name}_ids must be 2-D [M, n]")
+        n = ids.shape[1]
+        hist += (_arg(ids, name + "_ids", index, _I64, (M, n)), ids.stride(0), 0 if lens is None else _arg(lens, name + "_lens", index, _I32, (M,)), n)
+    pen = [0 if t is None else _arg(t, n, index, _F32, (M,)) for t, n in (
+        (repetition_penalty, "repetition_penalty"), (presence_penalty, "presence_penalty"), (frequency_penalty, "frequency_penalty"))]
+    pb = pv = ldb = nb = pa = lda = 0
     if (bias_ids is None) != (bias is None):
         raise ValueError("bias_ids and bias go together")
-    if bias is not None and bias.shape[1:] != (0,):
-        a.bias_ids, a.bias = _arg(bias_ids, "bias_ids", dev, torch.int32, (M, None)), _arg(bias, "bias", dev, f32, tuple(bias_ids.shape))
-        if bias_ids.stride(0) != bias.stride(0) and M > 1:
+    if bias is not None:
+        if bias.dim() != 2:
+            raise ValueError("bias must be 2-D [M, n]")
+        nb, ldb = bias.shape[1], bias.stride(0)
+        pb, pv = _arg(bias_ids, "bias_ids", index, _I32, (M, nb)), _arg(bias, "bias", index, _F32, (M, nb))
+        if M > 1 and bias_ids.stride(0) != ldb:
             raise ValueError("bias_ids and bias must have the same row stride")
-        a.ld_bias, a.n_bias = bias.stride(0), bias.shape[1]
     if allowed is not None:
-        a.allowed, a.ld_allowed = _arg(allowed, "allowed", dev, torch.int32, (M, (V + 31) // 32)), allowed.stride(0)
+        pa, lda = _arg(allowed, "allowed", index, _I32, (M, (V + 31) // 32)), allowed.stride(0)
     if M and V:
-        _call("mc_logits_process_f32", dev, C.byref(a))
+        _call("mc_logits_process_f32", index, _lib.LogitsArgsC(pl, logits.stride(0), po, ldo, M, V, *hist, *pen, pb, pv, ldb, nb, pa, lda))
     return out
