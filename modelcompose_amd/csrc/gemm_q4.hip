@@ -21,24 +21,260 @@ __device__ __forceinline__ void q4_store(const Q4Params& p, int m, int n, float 
     else ((bf16_t*)p.out)[m * p.ldo + n] = (bf16_t)y;
 }
 
-// a wave per output column; 8 codes (4 bytes) per lane and step
-__global__ __launch_bounds__(256) void linear_q4_kernel(Q4Params p) {
-    const int lane = threadIdx.x & 63, n = blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (n >= p.N) return;
-    for (int m = 0; m < p.M; ++m) {
-        float y = 0.f;
-        for (int k = lane * 8; k < p.K; k += 512) {
-            const uint32_t w = *(const uint32_t*)(p.codes + n * p.ldc + k / 2);
-            const int g = k >> p.gshift;
-            const float s = (float)p.scales[n * p.lds + g], z = p.zeros ? (float)p.zeros[n * p.ldz + g] : 8.f;
-            const bf16x8 x8 = *(const bf16x8*)(p.x + m * p.ldx + k);
-            float a = 0.f;
+typedef uint32_t u32_u __attribute__((aligned(1)));
+typedef uint32_t u32_u2 __attribute__((aligned(2)));
+typedef uint32_t u32x2_u2 __attribute__((ext_vector_type(2), aligned(2)));
+typedef uint16_t u16_u __attribute__((aligned(1)));
+
+constexpr int kQ4Waves = 8;
+constexpr int kQ4Block = 128;                    // columns of K that a wave takes at a time: 16 bytes of codes per lane
+
+// 8 codes of a word as 16-bit floats in column order.  A byte 0 .. 15 read as OCP e4m3 is its 2^-9 th part, exactly (the subnormals and the first binade of the
+// format have one spacing), and the conversion multiplies by its scale operand: 0.5 instructions per code, none for an offset.
+__device__ __forceinline__ bf16x8 q4_codes(uint32_t w) {
+    const uint32_t lo = w & 0x0f0f0f0fu, hi = (w >> 4) & 0x0f0f0f0fu;
+    const uint32_t a = __builtin_amdgcn_perm(hi, lo, 0x05010400u), b = __builtin_amdgcn_perm(hi, lo, 0x07030602u);
+#if MC_STORAGE_IS_F16
+    const u32x4 o = {__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(a, 512.f, false)), __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(a, 512.f, true)),
+                     __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(b, 512.f, false)), __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(b, 512.f, true))};
+#else
+    const u32x4 o = {__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(a, 512.f, false)), __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(a, 512.f, true)),
+                     __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(b, 512.f, false)), __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(b, 512.f, true))};
+#endif
+    return __builtin_bit_cast(bf16x8, o);
+}
+
+__device__ __forceinline__ float q4_scale(uint32_t bits) { return (float)__builtin_bit_cast(bf16_t, (uint16_t)bits); }
+
+// y[m][n] = sum over the groups g of s[n][g] (sum_k q[n][k] x[m][k] - z[n][g] sum_k x[m][k]), the inner sums on the matrix cores with the codes as exact integers: the
+// products are exact, the zero point is taken out of a sum of the same size (the codes reach 15, not 128 as with a biased exponent trick, so little is lost), the scale
+// is applied once per group in fp32.  sum_k x comes from the same instruction against a column of ones.
+//
+// A workgroup owns R blocks of 16 output columns over the whole of K; its 8 waves split K into contiguous chunks of 128-column blocks (a function of K alone), each wave
+// runs one chain in ascending k, the 8 chains are added in a fixed order: a row's bits depend neither on M nor on R.  Codes go from memory to registers once: 16 bytes
+// per lane, rows of 64 bytes side by side (consecutive rows of a row-major weight are one stream), a 4 x 4 transpose of words over the lane quarters
+// (v_permlane32_swap, v_permlane16_swap) turns them into the operands of four consecutive 32-column products.  x comes from the L2, once per workgroup.
+template <int MB, int R, int U, int UX, int GS, bool ZP, bool SMALL>
+__global__ __launch_bounds__(kQ4Waves * 64) void linear_q4_kernel(Q4Params p) {
+    constexpr int NG = 128 >> GS;                // groups per block
+    __shared__ __attribute__((aligned(16))) float red[4][R * MB][64][4];
+    const int tid = threadIdx.x, lane = tid & 63, c = lane & 15, g = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int blocks = (p.K + kQ4Block - 1) / kQ4Block, per = blocks / kQ4Waves, extra = blocks % kQ4Waves;
+    const int first = wave * per + min(wave, extra), count = per + (wave < extra ? 1 : 0);
+    const int tiles = (p.N + 15) >> 4;
+
+    const uint8_t* wrow[R]; const uint8_t* zrow[R]; const bf16_t* srow[R];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) a = fmaf((float)((w >> (4 * j)) & 15u) - z, (float)x8[j], a);
-            y = fmaf(a, s, y);
+    for (int r = 0; r < R; ++r) {
+        const int64_t n = min(min((int)blockIdx.x * R + r, tiles - 1) * 16 + c, p.N - 1);
+        wrow[r] = p.codes + n * p.ldc;
+        srow[r] = p.scales + n * p.lds;
+        zrow[r] = p.zeros + n * p.ldz;
+    }
+    const bf16_t* xrow[MB];
+#pragma unroll
+    for (int b = 0; b < MB; ++b) xrow[b] = p.x + (int64_t)min(b * 16 + c, p.M - 1) * p.ldx + 8 * g;
+
+    u32x4 wq[U][R];
+    uint32_t sq[U][R][(NG + 1) / 2], zq[U][R];
+    bf16x8 xq[UX][MB][4];
+    // i: block of the chunk; past its end the last block is read again and its scales are dropped.  No branches: they would cost the loads their order.
+    // The last block of K may be short (K % 128 = 32, 64 or 96).  Its missing pieces are whole groups (K is a multiple of the group): they are read from
+    // inside the row and get the scale 0.
+    const int groups = p.K >> GS;
+    auto load_w = [&](int u, int i) {
+        const int k = (first + min(i, count - 1)) * kQ4Block, last = ((p.K - k) >> 5) - 1;      // last: index of the last piece of 32 columns
+        const int q0 = SMALL ? 0 : min(k >> GS, groups - NG), missing = (k >> GS) - q0;          // (SMALL: fewer than NG groups in all)
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            wq[u][r] = __builtin_nontemporal_load((const u32x4*)(wrow[r] + (k >> 1) + 16 * min(g, last)));
+            const bf16_t* s = srow[r] + q0;
+            uint64_t sv = 0;
+            uint32_t zv = 0x08080808u;
+            if constexpr (SMALL) {
+#pragma unroll
+                for (int q = 0; q < NG; ++q) sv |= q < groups ? (uint64_t)*(const uint16_t*)(s + q) << (16 * q) : 0u;
+            } else if constexpr (NG == 1) sv = *(const uint16_t*)s;
+            else if constexpr (NG == 2) sv = *(const u32_u2*)s;
+            else { const u32x2 v = *(const u32x2_u2*)s; sv = v[0] | (uint64_t)v[1] << 32; }
+            if constexpr (ZP) {
+                const uint8_t* z = zrow[r] + q0;
+                zv = 0;
+                if constexpr (SMALL) {
+#pragma unroll
+                    for (int q = 0; q < NG; ++q) zv |= q < groups ? (uint32_t)z[q] << (8 * q) : 0u;
+                } else if constexpr (NG == 1) zv = *z;
+                else if constexpr (NG == 2) zv = *(const u16_u*)z;
+                else zv = *(const u32_u*)z;
+                if constexpr (NG > 1) zv >>= 8 * missing;
+            }
+            if constexpr (NG > 1) sv >>= 16 * missing;
+            if (U > 1) sv = i < count ? sv : 0u;
+            sq[u][r][0] = (uint32_t)sv;
+            if constexpr (NG > 2) sq[u][r][1] = (uint32_t)(sv >> 32);
+            zq[u][r] = zv;
         }
-        y = wave_sum(y);
-        if (lane == 0) q4_store(p, m, n, y);
+    };
+    auto load_x = [&](int u, int i) {
+        const int k = (first + min(i, count - 1)) * kQ4Block;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int kk = min(k + 32 * j, p.K - 32);
+#pragma unroll
+            for (int b = 0; b < MB; ++b) xq[u][b][j] = *(const bf16x8*)(xrow[b] + kk);
+        }
+    };
+
+    f32x4 acc[R][MB];
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+#pragma unroll
+        for (int b = 0; b < MB; ++b) acc[r][b] = (f32x4){0.f, 0.f, 0.f, 0.f};
+    bf16x8 ones;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) ones[j] = (bf16_t)1.f;
+
+    auto use = [&](int u, int ux) {
+        uint32_t w[R][4];
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            const auto a = __builtin_amdgcn_permlane32_swap(wq[u][r][0], wq[u][r][2], false, false);
+            const auto b = __builtin_amdgcn_permlane32_swap(wq[u][r][1], wq[u][r][3], false, false);
+            const auto d = __builtin_amdgcn_permlane16_swap(a[0], b[0], false, false);
+            const auto e = __builtin_amdgcn_permlane16_swap(a[1], b[1], false, false);
+            w[r][0] = d[0]; w[r][1] = d[1]; w[r][2] = e[0]; w[r][3] = e[1];
+        }
+        constexpr int JG = 4 / NG;               // products per group
+#pragma unroll
+        for (int q = 0; q < NG; ++q) {
+            f32x4 sx[MB], pr[R][MB];
+#pragma unroll
+            for (int b = 0; b < MB; ++b) sx[b] = (f32x4){0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int r = 0; r < R; ++r)
+#pragma unroll
+                for (int b = 0; b < MB; ++b) pr[r][b] = (f32x4){0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int j = q * JG; j < (q + 1) * JG; ++j) {
+#pragma unroll
+                for (int b = 0; b < MB; ++b) sx[b] = mc_mfma_16x16x32(xq[ux][b][j], ones, sx[b]);
+#pragma unroll
+                for (int r = 0; r < R; ++r) {
+                    const bf16x8 wf = q4_codes(w[r][j]);
+#pragma unroll
+                    for (int b = 0; b < MB; ++b) pr[r][b] = mc_mfma_16x16x32(xq[ux][b][j], wf, pr[r][b]);
+                }
+            }
+#pragma unroll
+            for (int r = 0; r < R; ++r) {
+                const float s = q4_scale(q & 1 ? sq[u][r][q >> 1] >> 16 : sq[u][r][q >> 1]), z = ZP ? (float)((zq[u][r] >> (8 * q)) & 255u) : 8.f;
+#pragma unroll
+                for (int b = 0; b < MB; ++b)
+#pragma unroll
+                    for (int t = 0; t < 4; ++t) acc[r][b][t] = fmaf(s, fmaf(-z, sx[b][t], pr[r][b][t]), acc[r][b][t]);
+            }
+            if constexpr (NG > 1) __builtin_amdgcn_sched_barrier(0);               // (groups interleaved by the scheduler spill)
+        }
+    };
+    if (count > 0) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) load_w(u, u);
+#pragma unroll
+        for (int u = 0; u < UX; ++u) load_x(u, u);
+        int i = 0;
+        for (; i + U < count; i += U) {
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                use(u, u % UX);
+                load_w(u, i + U + u);
+                load_x(u % UX, i + u + UX);
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            use(u, u % UX);
+            if constexpr (UX < U) { if (u + UX < U) load_x(u % UX, i + u + UX); }
+        }
+    }
+
+    // the 8 chains: (w + (w + 4)) for w = 0 .. 3, then those four in order
+    if (wave >= 4) {
+#pragma unroll
+        for (int r = 0; r < R; ++r)
+#pragma unroll
+            for (int b = 0; b < MB; ++b) *(f32x4*)&red[wave - 4][r * MB + b][lane][0] = acc[r][b];
+    }
+    __syncthreads();
+    if (wave < 4) {
+#pragma unroll
+        for (int r = 0; r < R; ++r)
+#pragma unroll
+            for (int b = 0; b < MB; ++b) {       // (slot `wave` is read and rewritten by this wave only)
+                acc[r][b] += *(f32x4*)&red[wave][r * MB + b][lane][0];
+                *(f32x4*)&red[wave][r * MB + b][lane][0] = acc[r][b];
+            }
+    }
+    __syncthreads();
+    for (int q = wave; q < R * MB; q += kQ4Waves) {
+        const int r = q / MB, b = q % MB;
+        f32x4 v = *(f32x4*)&red[0][q][lane][0];
+#pragma unroll
+        for (int w = 1; w < 4; ++w) v += *(f32x4*)&red[w][q][lane][0];
+        const int n = (blockIdx.x * R + r) * 16 + c;
+        if (n < p.N)
+#pragma unroll
+            for (int t = 0; t < 4; ++t) {
+                const int m = b * 16 + 4 * g + t;
+                if (m < p.M) q4_store(p, m, n, v[t]);
+            }
+    }
+}
+
+// column blocks per workgroup: a round (one workgroup per CU) costs what its workgroups take in - R x 8 K bytes of codes from memory, MB x 32 K bytes of x from the L2 at
+// a quarter of the price; the fewest round-bytes wins.  R * MB <= 12 keeps accumulators, rings and the 4 R MB KiB of LDS within two waves per SIMD.
+int q4_rows(int tiles, int mb) {
+    static const int most[4] = {6, 4, 3, 2};
+    int best = 1;
+    double cost = 1e30;
+    for (int R : {6, 4, 3, 2, 1}) {
+        if (R > most[mb - 1]) continue;
+        const double c = (double)(((tiles + R - 1) / R + 255) / 256) * (R + mb);
+        if (c < cost - 1e-9) { cost = c; best = R; }
+    }
+    return best;
+}
+
+template <int MB, int R, int U, int UX, int GS, bool SMALL>
+void q4_launch_z(const Q4Params& p, int grid, hipStream_t s) {
+    if (p.zeros) linear_q4_kernel<MB, R, U, UX, GS, true, SMALL><<<grid, kQ4Waves * 64, 0, s>>>(p);
+    else linear_q4_kernel<MB, R, U, UX, GS, false, SMALL><<<grid, kQ4Waves * 64, 0, s>>>(p);
+}
+
+template <int MB, int R, int U, int UX>
+void q4_launch_g(const Q4Params& p, int grid, hipStream_t s) {
+    if (p.gshift == 7) q4_launch_z<MB, R, U, UX, 7, false>(p, grid, s);
+    else if (p.gshift == 6) q4_launch_z<MB, R, U, UX, 6, false>(p, grid, s);
+    else q4_launch_z<MB, R, U, UX, 5, false>(p, grid, s);
+}
+
+template <int MB>
+void q4_launch(const Q4Params& p, hipStream_t s) {
+    const int tiles = (p.N + 15) / 16;
+    if (p.K < kQ4Block && p.gshift < 7) {            // less than one block of K
+        if (p.gshift == 6) q4_launch_z<MB, 1, 1, 1, 6, true>(p, tiles, s);
+        else q4_launch_z<MB, 1, 1, 1, 5, true>(p, tiles, s);
+        return;
+    }
+    const int R = q4_rows(tiles, MB), grid = (tiles + R - 1) / R;
+    if (R == 1) q4_launch_g<MB, 1, 4, MB == 1 ? 2 : 1>(p, grid, s);
+    else if (R == 2) q4_launch_g<MB, 2, 2, 1>(p, grid, s);
+    else if constexpr (MB <= 3) {
+        if (R == 3) q4_launch_g<MB, 3, 2, 1>(p, grid, s);
+        else if constexpr (MB <= 2) {
+            if (R == 4) q4_launch_g<MB, 4, 2, 1>(p, grid, s);
+            else if constexpr (MB == 1) q4_launch_g<1, 6, 2, 1>(p, grid, s);
+        }
     }
 }
 
@@ -113,7 +349,13 @@ extern "C" int mc_linear_q4_bf16(const void* x, int64_t ldx, const mc_q4_weight*
     if (M == 0) return 0;
     Q4Params p{(const bf16_t*)x, ldx, (const uint8_t*)w->codes, w->ldc, (const bf16_t*)w->scales, w->lds, (const uint8_t*)w->zeros, w->ldz, (const bf16_t*)bias,
                (const bf16_t*)residual, ldr, out, ldo, out_f32, M, w->N, w->K, group_shift(w->group)};
-    linear_q4_kernel<<<(w->N + 3) / 4, 256, 0, (hipStream_t)stream>>>(p);
+    hipStream_t s = (hipStream_t)stream;
+    switch ((M + 15) / 16) {
+        case 1: q4_launch<1>(p, s); break;
+        case 2: q4_launch<2>(p, s); break;
+        case 3: q4_launch<3>(p, s); break;
+        default: q4_launch<4>(p, s); break;
+    }
     MC_CHECK_LAUNCH();
     return 0;
 }
