@@ -21,9 +21,11 @@ __device__ __forceinline__ void q4_store(const Q4Params& p, int m, int n, float 
     else ((bf16_t*)p.out)[m * p.ldo + n] = (bf16_t)y;
 }
 
-typedef uint32_t u32_u __attribute__((aligned(1)));
 typedef uint32_t u32_u2 __attribute__((aligned(2)));
 typedef uint32_t u32x2_u2 __attribute__((ext_vector_type(2), aligned(2)));
+typedef uint32_t u32x4_u2 __attribute__((ext_vector_type(4), aligned(2)));
+typedef uint32_t u32_u __attribute__((aligned(1)));
+typedef uint32_t u32x2_u __attribute__((ext_vector_type(2), aligned(1)));
 typedef uint16_t u16_u __attribute__((aligned(1)));
 
 constexpr int kQ4Waves = 8;
@@ -54,7 +56,9 @@ __device__ __forceinline__ float q4_scale(uint32_t bits) { return (float)__built
 // runs one chain in ascending k, the 8 chains are added in a fixed order: a row's bits depend neither on M nor on R.  Codes go from memory to registers once: 16 bytes
 // per lane, rows of 64 bytes side by side (consecutive rows of a row-major weight are one stream), a 4 x 4 transpose of words over the lane quarters
 // (v_permlane32_swap, v_permlane16_swap) turns them into the operands of four consecutive 32-column products.  x comes from the L2, once per workgroup.
-template <int MB, int R, int U, int UX, int GS, bool ZP, bool SMALL>
+// Scales and zero points of 8 blocks are read at once, two blocks' per lane quarter, and handed round by ds_bpermute: a load of two bytes from each of 16 rows
+// costs the memory pipeline as much as 1 KiB of codes (8 x 32000 x 4096, groups of 64: 36 us with a scale and a zero load per block, XXX so).
+template <int MB, int R, int U, int UX, int GS, bool ZP>
 __global__ __launch_bounds__(kQ4Waves * 64) void linear_q4_kernel(Q4Params p) {
     constexpr int NG = 128 >> GS;                // groups per block
     __shared__ __attribute__((aligned(16))) float red[4][R * MB][64][4];
@@ -77,43 +81,48 @@ __global__ __launch_bounds__(kQ4Waves * 64) void linear_q4_kernel(Q4Params p) {
     for (int b = 0; b < MB; ++b) xrow[b] = p.x + (int64_t)min(b * 16 + c, p.M - 1) * p.ldx + 8 * g;
 
     u32x4 wq[U][R];
-    uint32_t sq[U][R][(NG + 1) / 2], zq[U][R];
     bf16x8 xq[UX][MB][4];
-    // i: block of the chunk; past its end the last block is read again and its scales are dropped.  No branches: they would cost the loads their order.
-    // The last block of K may be short (K % 128 = 32, 64 or 96).  Its missing pieces are whole groups (K is a multiple of the group): they are read from
-    // inside the row and get the scale 0.
-    const int groups = p.K >> GS;
+    // i: block of the chunk; past its end the last block is read again (and its scales are dropped).  The last block of K may be short (K % 128 = 32, 64 or 96): its
+    // missing pieces are whole groups (K is a multiple of the group), are read from inside the row and have the scale 0.  No branches: they would cost the
+    // loads their order.
     auto load_w = [&](int u, int i) {
         const int k = (first + min(i, count - 1)) * kQ4Block, last = ((p.K - k) >> 5) - 1;      // last: index of the last piece of 32 columns
-        const int q0 = SMALL ? 0 : min(k >> GS, groups - NG), missing = (k >> GS) - q0;          // (SMALL: fewer than NG groups in all)
 #pragma unroll
-        for (int r = 0; r < R; ++r) {
-            wq[u][r] = __builtin_nontemporal_load((const u32x4*)(wrow[r] + (k >> 1) + 16 * min(g, last)));
-            const bf16_t* s = srow[r] + q0;
-            uint64_t sv = 0;
-            uint32_t zv = 0x08080808u;
-            if constexpr (SMALL) {
+        for (int r = 0; r < R; ++r) wq[u][r] = __builtin_nontemporal_load((const u32x4*)(wrow[r] + (k >> 1) + 16 * min(g, last)));
+    };
+    // scales and zero points of blocks 8 t .. 8 t + 7 of the chunk: quarter g holds those of blocks 8 t + 2 g and the next, 2 NG of them
+    constexpr int ZW = NG == 4 ? 2 : 1;
+    struct Scales { uint32_t s[R][NG], z[R][ZW]; };
+    const int groups = p.K >> GS;
+    auto load_s = [&](Scales& o, int t) {
+        const int q0 = (first + 8 * t + 2 * g) * NG;
+        if ((first + 8 * t + 8) * NG <= groups) {
 #pragma unroll
-                for (int q = 0; q < NG; ++q) sv |= q < groups ? (uint64_t)*(const uint16_t*)(s + q) << (16 * q) : 0u;
-            } else if constexpr (NG == 1) sv = *(const uint16_t*)s;
-            else if constexpr (NG == 2) sv = *(const u32_u2*)s;
-            else { const u32x2 v = *(const u32x2_u2*)s; sv = v[0] | (uint64_t)v[1] << 32; }
-            if constexpr (ZP) {
+            for (int r = 0; r < R; ++r) {
+                const bf16_t* s = srow[r] + q0;
                 const uint8_t* z = zrow[r] + q0;
-                zv = 0;
-                if constexpr (SMALL) {
+                if constexpr (NG == 1) { o.s[r][0] = *(const u32_u2*)s; if (ZP) o.z[r][0] = *(const u16_u*)z; }
+                else if constexpr (NG == 2) { const u32x2 v = *(const u32x2_u2*)s; o.s[r][0] = v[0]; o.s[r][1] = v[1]; if (ZP) o.z[r][0] = *(const u32_u*)z; }
+                else {
+                    const u32x4 v = *(const u32x4_u2*)s;
 #pragma unroll
-                    for (int q = 0; q < NG; ++q) zv |= q < groups ? (uint32_t)z[q] << (8 * q) : 0u;
-                } else if constexpr (NG == 1) zv = *z;
-                else if constexpr (NG == 2) zv = *(const u16_u*)z;
-                else zv = *(const u32_u*)z;
-                if constexpr (NG > 1) zv >>= 8 * missing;
+                    for (int q = 0; q < 4; ++q) o.s[r][q] = v[q];
+                    if (ZP) { const u32x2 y = *(const u32x2_u*)z; o.z[r][0] = y[0]; o.z[r][1] = y[1]; }
+                }
             }
-            if constexpr (NG > 1) sv >>= 16 * missing;
-            if (U > 1) sv = i < count ? sv : 0u;
-            sq[u][r][0] = (uint32_t)sv;
-            if constexpr (NG > 2) sq[u][r][1] = (uint32_t)(sv >> 32);
-            zq[u][r] = zv;
+        } else {                                     // the end of the row: what there is
+#pragma unroll
+            for (int r = 0; r < R; ++r) {
+#pragma unroll
+                for (int q = 0; q < ZW; ++q) o.z[r][q] = 0;
+#pragma unroll
+                for (int q = 0; q < 2 * NG; ++q) {
+                    const int at = min(q0 + q, groups - 1);
+                    const uint32_t v = q0 + q < groups ? *(const uint16_t*)(srow[r] + at) : 0u;
+                    if (q & 1) o.s[r][q >> 1] |= v << 16; else o.s[r][q >> 1] = v;
+                    if (ZP) o.z[r][q >> 2] |= (uint32_t)zrow[r][at] << (8 * (q & 3));
+                }
+            }
         }
     };
     auto load_x = [&](int u, int i) {
@@ -135,8 +144,22 @@ __global__ __launch_bounds__(kQ4Waves * 64) void linear_q4_kernel(Q4Params p) {
 #pragma unroll
     for (int j = 0; j < 8; ++j) ones[j] = (bf16_t)1.f;
 
-    auto use = [&](int u, int ux) {
-        uint32_t w[R][4];
+    // odd: parity of block i (of the chunk)
+    auto use = [&](const Scales& o, int u, int ux, int odd, int i) {
+        const int from = 4 * c + 64 * ((i & 7) >> 1);
+        uint32_t sv[R][(NG + 1) / 2], zv[R], w[R][4];
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+#pragma unroll
+            for (int q = 0; q < (NG + 1) / 2; ++q) {
+                const uint32_t v = (uint32_t)__builtin_amdgcn_ds_bpermute(from, (int)o.s[r][NG == 1 ? 0 : odd * (NG / 2) + q]);
+                sv[r][q] = i < count ? (NG == 1 && odd ? v >> 16 : v) : 0u;
+            }
+            if (ZP) {
+                zv[r] = (uint32_t)__builtin_amdgcn_ds_bpermute(from, (int)o.z[r][NG == 4 ? odd : 0]);
+                if (NG < 4 && odd) zv[r] >>= 8 * NG;
+            }
+        }
 #pragma unroll
         for (int r = 0; r < R; ++r) {
             const auto a = __builtin_amdgcn_permlane32_swap(wq[u][r][0], wq[u][r][2], false, false);
@@ -168,7 +191,7 @@ __global__ __launch_bounds__(kQ4Waves * 64) void linear_q4_kernel(Q4Params p) {
             }
 #pragma unroll
             for (int r = 0; r < R; ++r) {
-                const float s = q4_scale(q & 1 ? sq[u][r][q >> 1] >> 16 : sq[u][r][q >> 1]), z = ZP ? (float)((zq[u][r] >> (8 * q)) & 255u) : 8.f;
+                const float s = q4_scale(q & 1 ? sv[r][q >> 1] >> 16 : sv[r][q >> 1]), z = ZP ? (float)((zv[r] >> (8 * q)) & 255u) : 8.f;
 #pragma unroll
                 for (int b = 0; b < MB; ++b)
 #pragma unroll
@@ -178,23 +201,34 @@ __global__ __launch_bounds__(kQ4Waves * 64) void linear_q4_kernel(Q4Params p) {
         }
     };
     if (count > 0) {
+        Scales cur, nxt;
+        load_s(cur, 0);
 #pragma unroll
         for (int u = 0; u < U; ++u) load_w(u, u);
 #pragma unroll
         for (int u = 0; u < UX; ++u) load_x(u, u);
+        if (8 < count) load_s(nxt, 1);
         int i = 0;
-        for (; i + U < count; i += U) {
+        auto turn = [&] {                        // every 8 blocks the next scales
+            if (i && !(i & 7)) {
+                cur = nxt;
+                if (i + 8 < count) load_s(nxt, (i >> 3) + 1);
+            }
+        };
+        for (; i + U < count; i += U) {          // (U divides 8)
+            turn();
 #pragma unroll
             for (int u = 0; u < U; ++u) {
-                use(u, u % UX);
+                use(cur, u, u % UX, u & 1, i + u);
                 load_w(u, i + U + u);
                 load_x(u % UX, i + u + UX);
             }
         }
+        turn();
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            use(u, u % UX);
-            if constexpr (UX < U) { if (u + UX < U) load_x(u % UX, i + u + UX); }
+            use(cur, u, u % UX, u & 1, i + u);
+            if (u + UX < U) load_x(u % UX, i + u + UX);
         }
     }
 
@@ -245,27 +279,22 @@ int q4_rows(int tiles, int mb) {
     return best;
 }
 
-template <int MB, int R, int U, int UX, int GS, bool SMALL>
+template <int MB, int R, int U, int UX, int GS>
 void q4_launch_z(const Q4Params& p, int grid, hipStream_t s) {
-    if (p.zeros) linear_q4_kernel<MB, R, U, UX, GS, true, SMALL><<<grid, kQ4Waves * 64, 0, s>>>(p);
-    else linear_q4_kernel<MB, R, U, UX, GS, false, SMALL><<<grid, kQ4Waves * 64, 0, s>>>(p);
+    if (p.zeros) linear_q4_kernel<MB, R, U, UX, GS, true><<<grid, kQ4Waves * 64, 0, s>>>(p);
+    else linear_q4_kernel<MB, R, U, UX, GS, false><<<grid, kQ4Waves * 64, 0, s>>>(p);
 }
 
 template <int MB, int R, int U, int UX>
 void q4_launch_g(const Q4Params& p, int grid, hipStream_t s) {
-    if (p.gshift == 7) q4_launch_z<MB, R, U, UX, 7, false>(p, grid, s);
-    else if (p.gshift == 6) q4_launch_z<MB, R, U, UX, 6, false>(p, grid, s);
-    else q4_launch_z<MB, R, U, UX, 5, false>(p, grid, s);
+    if (p.gshift == 7) q4_launch_z<MB, R, U, UX, 7>(p, grid, s);
+    else if (p.gshift == 6) q4_launch_z<MB, R, U, UX, 6>(p, grid, s);
+    else q4_launch_z<MB, R, U, UX, 5>(p, grid, s);
 }
 
 template <int MB>
 void q4_launch(const Q4Params& p, hipStream_t s) {
     const int tiles = (p.N + 15) / 16;
-    if (p.K < kQ4Block && p.gshift < 7) {            // less than one block of K
-        if (p.gshift == 6) q4_launch_z<MB, 1, 1, 1, 6, true>(p, tiles, s);
-        else q4_launch_z<MB, 1, 1, 1, 5, true>(p, tiles, s);
-        return;
-    }
     const int R = q4_rows(tiles, MB), grid = (tiles + R - 1) / R;
     if (R == 1) q4_launch_g<MB, 1, 4, MB == 1 ? 2 : 1>(p, grid, s);
     else if (R == 2) q4_launch_g<MB, 2, 2, 1>(p, grid, s);
