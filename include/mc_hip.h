@@ -404,7 +404,7 @@ typedef struct mc_logits_args {
     const int64_t* prompt_ids; int64_t ld_prompt; const int32_t* prompt_lens; int prompt_cols;
     const int64_t* output_ids; int64_t ld_output; const int32_t* output_lens; int output_cols;
     const float* repetition; const float* presence; const float* frequency;   /* [M] each */
-    const int32_t* bias_ids; const float* bias; int64_t ld_bias; int n_bias;   /* [M, n_bias], n_bias <= 4096 */
+    const int32_t* bias_ids; const float* bias; int64_t ld_bias; int n_bias;   /* [M, n_bias], n_bias <= 1024 */
     const int32_t* allowed; int64_t ld_allowed;                               /* [M, ceil(V / 32)] */
 } mc_logits_args;
 int mc_logits_process_f32(const mc_logits_args* args, void* stream);
@@ -419,7 +419,9 @@ typedef struct mc_q4_weight {
 /* out[M, N] = x[M, K] W^T (+ bias) (+ residual): at most 64 rows; out 16-bit, or fp32 with out_f32.  Codes are multiplied as exact integers and summed in
  * fp32 per group, then scaled; a row's result does not depend on M. */
 int mc_linear_q4_bf16(const void* x, int64_t ldx, const mc_q4_weight* w, const void* bias, const void* residual, int64_t ldr, void* out, int64_t ldo,
-                      int M, int out_f32, void* stream);
+                      int M, int out_f32, void* workspace, void* stream);
+/* scratch of that call (0 up to 16 rows: workspace may be NULL), 16-byte aligned */
+int mc_linear_q4_workspace_bytes(int M, int K, int64_t* bytes);
 /* codes [N, K / 2], scales [N, K / group] (and zeros, unless NULL: symmetric codes around 8) of a 16-bit weight, all contiguous */
 int mc_quantize_q4_bf16(const void* w, int64_t ldw, void* codes, void* scales, void* zeros, int N, int K, int group, void* stream);
 /* the packed 16-bit form (mc_packed_weight_elems) for launches of more than 64 rows */

@@ -176,7 +176,8 @@ class Kv8CacheC(C.Structure):
 
 _SIGS.update({
     "mc_logits_process_f32": [C.POINTER(LogitsArgsC), c_p],
-    "mc_linear_q4_bf16": [c_p, c_l, C.POINTER(Q4WeightC), c_p, c_p, c_l, c_p, c_l, c_i, c_i, c_p],
+    "mc_linear_q4_bf16": [c_p, c_l, C.POINTER(Q4WeightC), c_p, c_p, c_l, c_p, c_l, c_i, c_i, c_p, c_p],
+    "mc_linear_q4_workspace_bytes": [c_i, c_i, C.POINTER(c_l)],
     "mc_quantize_q4_bf16": [c_p, c_l, c_p, c_p, c_p, c_i, c_i, c_i, c_p],
     "mc_dequantize_q4_bf16": [C.POINTER(Q4WeightC), c_p, c_p],
     "mc_rope_kv8": [c_p, c_l, c_p, c_p, c_p, c_p, c_p, c_i, c_p, C.POINTER(Kv8CacheC), c_i, c_i, c_i, c_p],

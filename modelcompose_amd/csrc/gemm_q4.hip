@@ -12,6 +12,7 @@ struct Q4Params {
     const bf16_t* bias; const bf16_t* residual; int64_t ldr;
     void* out; int64_t ldo; int out_f32;
     int M, N, K, gshift;                     // group = 1 << gshift
+    const bf16_t* xp;                        // x in operand order (pack_x_kernel), for more than 16 rows
 };
 
 __device__ __forceinline__ void q4_store(const Q4Params& p, int m, int n, float y) {
@@ -28,7 +29,6 @@ typedef uint32_t u32_u __attribute__((aligned(1)));
 typedef uint32_t u32x2_u __attribute__((ext_vector_type(2), aligned(1)));
 typedef uint16_t u16_u __attribute__((aligned(1)));
 
-constexpr int kQ4Waves = 8;
 constexpr int kQ4Block = 128;                    // columns of K that a wave takes at a time: 16 bytes of codes per lane
 
 // 8 codes of a word as 16-bit floats in column order.  A byte 0 .. 15 read as OCP e4m3 is its 2^-9 th part, exactly (the subnormals and the first binade of the
@@ -52,19 +52,21 @@ __device__ __forceinline__ float q4_scale(uint32_t bits) { return (float)__built
 // products are exact, the zero point is taken out of a sum of the same size (the codes reach 15, not 128 as with a biased exponent trick, so little is lost), the scale
 // is applied once per group in fp32.  sum_k x comes from the same instruction against a column of ones.
 //
-// A workgroup owns R blocks of 16 output columns over the whole of K; its 8 waves split K into contiguous chunks of 128-column blocks (a function of K alone), each wave
-// runs one chain in ascending k, the 8 chains are added in a fixed order: a row's bits depend neither on M nor on R.  Codes go from memory to registers once: 16 bytes
+// A workgroup owns R blocks of 16 output columns over the whole of K; its W waves split K into contiguous chunks of 128-column blocks (a function of K and N), each wave
+// runs one chain in ascending k, the W chains are added in a fixed order: a row's bits depend neither on M nor on R.  Codes go from memory to registers once: 16 bytes
 // per lane, rows of 64 bytes side by side (consecutive rows of a row-major weight are one stream), a 4 x 4 transpose of words over the lane quarters
-// (v_permlane32_swap, v_permlane16_swap) turns them into the operands of four consecutive 32-column products.  x comes from the L2, once per workgroup.
+// (v_permlane32_swap, v_permlane16_swap) turns them into the operands of four consecutive 32-column products.  x comes from the L2, once per workgroup (over 16 rows in operand order: q4_pack_x_kernel).
 // Scales and zero points of 8 blocks are read at once, two blocks' per lane quarter, and handed round by ds_bpermute: a load of two bytes from each of 16 rows
-// costs the memory pipeline as much as 1 KiB of codes (8 x 32000 x 4096, groups of 64: 36 us with a scale and a zero load per block, XXX so).
-template <int MB, int R, int U, int UX, int GS, bool ZP>
-__global__ __launch_bounds__(kQ4Waves * 64) void linear_q4_kernel(Q4Params p) {
+// costs the memory pipeline as much as 1 KiB of codes (8 x 32000 x 4096, groups of 64: 36 us with a scale and a zero load per block, 31 so,
+// the rest of the kernel being the same).
+template <int W, int MB, int R, int U, int UX, int GS, bool ZP>
+__global__ __launch_bounds__(W * 64) void linear_q4_kernel(Q4Params p) {
     constexpr int NG = 128 >> GS;                // groups per block
-    __shared__ __attribute__((aligned(16))) float red[4][R * MB][64][4];
+    constexpr int H = W / 2;
+    __shared__ __attribute__((aligned(16))) float red[H][R * MB][64][4];
     const int tid = threadIdx.x, lane = tid & 63, c = lane & 15, g = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int blocks = (p.K + kQ4Block - 1) / kQ4Block, per = blocks / kQ4Waves, extra = blocks % kQ4Waves;
+    const int blocks = (p.K + kQ4Block - 1) / kQ4Block, per = blocks / W, extra = blocks % W;
     const int first = wave * per + min(wave, extra), count = per + (wave < extra ? 1 : 0);
     const int tiles = (p.N + 15) >> 4;
 
@@ -76,9 +78,7 @@ __global__ __launch_bounds__(kQ4Waves * 64) void linear_q4_kernel(Q4Params p) {
         srow[r] = p.scales + n * p.lds;
         zrow[r] = p.zeros + n * p.ldz;
     }
-    const bf16_t* xrow[MB];
-#pragma unroll
-    for (int b = 0; b < MB; ++b) xrow[b] = p.x + (int64_t)min(b * 16 + c, p.M - 1) * p.ldx + 8 * g;
+    const bf16_t* xrow = MB > 1 ? p.xp + lane * 8 : p.x + (int64_t)min(c, p.M - 1) * p.ldx + 8 * g;
 
     u32x4 wq[U][R];
     bf16x8 xq[UX][MB][4];
@@ -131,7 +131,7 @@ __global__ __launch_bounds__(kQ4Waves * 64) void linear_q4_kernel(Q4Params p) {
         for (int j = 0; j < 4; ++j) {
             const int kk = min(k + 32 * j, p.K - 32);
 #pragma unroll
-            for (int b = 0; b < MB; ++b) xq[u][b][j] = *(const bf16x8*)(xrow[b] + kk);
+            for (int b = 0; b < MB; ++b) xq[u][b][j] = *(const bf16x8*)(xrow + (MB > 1 ? ((int64_t)(kk >> 5) * MB + b) * 512 : kk));
         }
     };
 
@@ -232,15 +232,15 @@ __global__ __launch_bounds__(kQ4Waves * 64) void linear_q4_kernel(Q4Params p) {
         }
     }
 
-    // the 8 chains: (w + (w + 4)) for w = 0 .. 3, then those four in order
-    if (wave >= 4) {
+    // the W chains: (w + (w + W / 2)) for the lower half, then those in order
+    if (wave >= H) {
 #pragma unroll
         for (int r = 0; r < R; ++r)
 #pragma unroll
-            for (int b = 0; b < MB; ++b) *(f32x4*)&red[wave - 4][r * MB + b][lane][0] = acc[r][b];
+            for (int b = 0; b < MB; ++b) *(f32x4*)&red[wave - H][r * MB + b][lane][0] = acc[r][b];
     }
     __syncthreads();
-    if (wave < 4) {
+    if (wave < H) {
 #pragma unroll
         for (int r = 0; r < R; ++r)
 #pragma unroll
@@ -250,11 +250,11 @@ __global__ __launch_bounds__(kQ4Waves * 64) void linear_q4_kernel(Q4Params p) {
             }
     }
     __syncthreads();
-    for (int q = wave; q < R * MB; q += kQ4Waves) {
+    for (int q = wave; q < R * MB; q += W) {
         const int r = q / MB, b = q % MB;
         f32x4 v = *(f32x4*)&red[0][q][lane][0];
 #pragma unroll
-        for (int w = 1; w < 4; ++w) v += *(f32x4*)&red[w][q][lane][0];
+        for (int w = 1; w < H; ++w) v += *(f32x4*)&red[w][q][lane][0];
         const int n = (blockIdx.x * R + r) * 16 + c;
         if (n < p.N)
 #pragma unroll
@@ -265,46 +265,41 @@ __global__ __launch_bounds__(kQ4Waves * 64) void linear_q4_kernel(Q4Params p) {
     }
 }
 
-// column blocks per workgroup: a round (one workgroup per CU) costs what its workgroups take in - R x 8 K bytes of codes from memory, MB x 32 K bytes of x from the L2 at
-// a quarter of the price; the fewest round-bytes wins.  R * MB <= 12 keeps accumulators, rings and the 4 R MB KiB of LDS within two waves per SIMD.
-int q4_rows(int tiles, int mb) {
-    static const int most[4] = {6, 4, 3, 2};
-    int best = 1;
-    double cost = 1e30;
-    for (int R : {6, 4, 3, 2, 1}) {
-        if (R > most[mb - 1]) continue;
-        const double c = (double)(((tiles + R - 1) / R + 255) / 256) * (R + mb);
-        if (c < cost - 1e-9) { cost = c; best = R; }
-    }
-    return best;
+// x [M, K] in operand order, [K / 32][MB][64 lanes][8], rows from M on zero: the rows of x lie a power of two apart as a rule, and the 16 rows of an operand, read by every
+// workgroup at once, then come from few channels of the L2
+__global__ __launch_bounds__(256) void q4_pack_x_kernel(const bf16_t* x, int64_t ldx, bf16_t* xp, int M, int K, int mb) {
+    const int i = blockIdx.x * 256 + threadIdx.x, lane = i & 63, f = i >> 6, kb = f / mb, b = f % mb;
+    if (kb * 32 >= K) return;
+    const int m = b * 16 + (lane & 15);
+    bf16x8 v = {};
+    if (m < M) v = *(const bf16x8*)(x + (int64_t)m * ldx + kb * 32 + 8 * (lane >> 4));
+    *(bf16x8*)(xp + (int64_t)i * 8) = v;
 }
 
-template <int MB, int R, int U, int UX, int GS>
-void q4_launch_z(const Q4Params& p, int grid, hipStream_t s) {
-    if (p.zeros) linear_q4_kernel<MB, R, U, UX, GS, true><<<grid, kQ4Waves * 64, 0, s>>>(p);
-    else linear_q4_kernel<MB, R, U, UX, GS, false><<<grid, kQ4Waves * 64, 0, s>>>(p);
+template <int W, int MB, int R, int U, int UX, int GS>
+void q4_launch_z(const Q4Params& p, hipStream_t s) {
+    const int grid = ((p.N + 15) / 16 + R - 1) / R;
+    if (p.zeros) linear_q4_kernel<W, MB, R, U, UX, GS, true><<<grid, W * 64, 0, s>>>(p);
+    else linear_q4_kernel<W, MB, R, U, UX, GS, false><<<grid, W * 64, 0, s>>>(p);
 }
 
-template <int MB, int R, int U, int UX>
-void q4_launch_g(const Q4Params& p, int grid, hipStream_t s) {
-    if (p.gshift == 7) q4_launch_z<MB, R, U, UX, 7>(p, grid, s);
-    else if (p.gshift == 6) q4_launch_z<MB, R, U, UX, 6>(p, grid, s);
-    else q4_launch_z<MB, R, U, UX, 5>(p, grid, s);
+template <int W, int MB, int R, int U, int UX>
+void q4_launch_g(const Q4Params& p, hipStream_t s) {
+    if (p.gshift == 7) q4_launch_z<W, MB, R, U, UX, 7>(p, s);
+    else if (p.gshift == 6) q4_launch_z<W, MB, R, U, UX, 6>(p, s);
+    else q4_launch_z<W, MB, R, U, UX, 5>(p, s);
 }
 
+// R blocks of 16 columns per workgroup: enough to bring the workgroups down to one per CU, up to 3 (x is read once per workgroup: 48 x 12288 x 4096 takes 25 us with R = 1, 23
+// with 2, 19 with 3; 1 x 4096 x 4096, whose 256 blocks just fill the chip, 5.2, 6.7 and 8.5).  Waves per workgroup, a function of N alone because it decides the order of the
+// sums: 8 up to 512 blocks, where longer chains leave the chip idle (1 x 4096 x 4096: 5.2 against 6.2 us), 4 above, where shorter ones spend their time starting and
+// ending (8 x 32000 x 4096: 24 against 34 us).
 template <int MB>
 void q4_launch(const Q4Params& p, hipStream_t s) {
     const int tiles = (p.N + 15) / 16;
-    const int R = q4_rows(tiles, MB), grid = (tiles + R - 1) / R;
-    if (R == 1) q4_launch_g<MB, 1, 4, MB == 1 ? 2 : 1>(p, grid, s);
-    else if (R == 2) q4_launch_g<MB, 2, 2, 1>(p, grid, s);
-    else if constexpr (MB <= 3) {
-        if (R == 3) q4_launch_g<MB, 3, 2, 1>(p, grid, s);
-        else if constexpr (MB <= 2) {
-            if (R == 4) q4_launch_g<MB, 4, 2, 1>(p, grid, s);
-            else if constexpr (MB == 1) q4_launch_g<1, 6, 2, 1>(p, grid, s);
-        }
-    }
+    if (tiles <= 256) q4_launch_g<8, MB, 1, 2, 1>(p, s);
+    else if (tiles <= 512) q4_launch_g<8, MB, 2, 2, 1>(p, s);
+    else q4_launch_g<4, MB, 3, 2, 1>(p, s);
 }
 
 // ---- weights ----------------------------------------------------------------------------------------------------------------------
@@ -370,22 +365,34 @@ int check_weight(const mc_q4_weight* w, const char* who) {
 }  // namespace
 
 extern "C" int mc_linear_q4_bf16(const void* x, int64_t ldx, const mc_q4_weight* w, const void* bias, const void* residual, int64_t ldr, void* out, int64_t ldo,
-                                 int M, int out_f32, void* stream) {
+                                 int M, int out_f32, void* workspace, void* stream) {
     if (int e = check_weight(w, "mc_linear_q4_bf16")) return e;
     MC_CHECK_ARG(M >= 0 && M <= 64, "mc_linear_q4_bf16: M = %d rows (at most 64: larger ones take the 16-bit form, mc_dequantize_q4_bf16)", M);
     MC_CHECK_ARG(x && out && (uintptr_t)x % 16 == 0 && ldx % 8 == 0 && (M <= 1 || ldx >= w->K), "mc_linear_q4_bf16: rows of x must be 16-byte aligned");
     MC_CHECK_ARG((uintptr_t)out % (out_f32 ? 4 : 2) == 0 && (M <= 1 || (ldo >= w->N && (!residual || ldr >= w->N))), "mc_linear_q4_bf16: bad output or residual rows");
     if (M == 0) return 0;
     Q4Params p{(const bf16_t*)x, ldx, (const uint8_t*)w->codes, w->ldc, (const bf16_t*)w->scales, w->lds, (const uint8_t*)w->zeros, w->ldz, (const bf16_t*)bias,
-               (const bf16_t*)residual, ldr, out, ldo, out_f32, M, w->N, w->K, group_shift(w->group)};
+               (const bf16_t*)residual, ldr, out, ldo, out_f32, M, w->N, w->K, group_shift(w->group), nullptr};
     hipStream_t s = (hipStream_t)stream;
-    switch ((M + 15) / 16) {
+    const int mb = (M + 15) / 16;
+    if (mb > 1) {
+        MC_CHECK_ARG(workspace && (uintptr_t)workspace % 16 == 0, "mc_linear_q4_bf16: more than 16 rows need a workspace of mc_linear_q4_workspace_bytes, 16-byte aligned");
+        p.xp = (const bf16_t*)workspace;
+        q4_pack_x_kernel<<<(w->K / 32 * mb * 64 + 255) / 256, 256, 0, s>>>(p.x, ldx, (bf16_t*)workspace, M, w->K, mb);
+    }
+    switch (mb) {
         case 1: q4_launch<1>(p, s); break;
         case 2: q4_launch<2>(p, s); break;
         case 3: q4_launch<3>(p, s); break;
         default: q4_launch<4>(p, s); break;
     }
     MC_CHECK_LAUNCH();
+    return 0;
+}
+
+extern "C" int mc_linear_q4_workspace_bytes(int M, int K, int64_t* bytes) {
+    MC_CHECK_ARG(bytes && M >= 0 && M <= 64 && K > 0, "mc_linear_q4_workspace_bytes: bad arguments");
+    *bytes = M > 16 ? (int64_t)((M + 15) / 16) * 16 * K * 2 : 0;
     return 0;
 }
 

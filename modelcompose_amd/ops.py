@@ -742,8 +742,10 @@ def linear_q4(x: torch.Tensor, w: Q4Weight, residual: Optional[torch.Tensor] = N
         po, ldo = _arg(out, "out", index, dt, (M, N)), out.stride(0)
     pr, ldr = (0, 0) if residual is None else (_arg(residual, "residual", index, BF16, (M, N)), residual.stride(0))
     if M:
+        # (mc_linear_q4_workspace_bytes)
+        ws = torch.empty((M + 15) // 16 * 16 * w.K, dtype=BF16, device=x.device) if M > 16 else None
         _call("mc_linear_q4_bf16", index, px, x.stride(0) if M > 1 else w.K, w._c, w.bias.data_ptr() if bias and w.bias is not None else 0, pr, ldr, po, ldo, M,
-              1 if out_f32 else 0)
+              1 if out_f32 else 0, 0 if ws is None else ws.data_ptr())
     return out
 
 

@@ -68,12 +68,18 @@ def test_bad_q4_calls(lib):
         d = dict(codes=4096, ldc=128, scales=4096, lds=2, zeros=0, ldz=0, N=8, K=256, group=128)
         d.update(kw)
         return lib.Q4WeightC(*[d[n] for n, _ in lib.Q4WeightC._fields_])
-    call = lambda ww, M=4, ldx=256, x=one, ldo=8, out=one: L.mc_linear_q4_bf16(x, ldx, C.byref(ww), None, None, 0, out, ldo, M, 0, None)
+    call = lambda ww, M=4, ldx=256, x=one, ldo=8, out=one, ws=None: L.mc_linear_q4_bf16(x, ldx, C.byref(ww), None, None, 0, out, ldo, M, 0, ws, None)
     for bad, text in ((dict(codes=0), "null weight"), (dict(group=96), "group 96"), (dict(K=192), "multiple"), (dict(N=0), "positive"), (dict(ldc=120), "16-byte"), (dict(ldc=112), "16-byte"),
                       (dict(codes=4100), "16-byte"), (dict(lds=1), "scales or zeros"), (dict(zeros=4096, ldz=1), "scales or zeros")):
         refused(lib, call(w(**bad)), text)
         refused(lib, L.mc_dequantize_q4_bf16(C.byref(w(**bad)), one, None), text)
     refused(lib, call(w(), M=65), "at most 64")
+    refused(lib, call(w(), M=17), "workspace")
+    refused(lib, call(w(), M=17, ws=4104), "workspace")
+    n = C.c_int64(-1)
+    assert L.mc_linear_q4_workspace_bytes(16, 256, C.byref(n)) == 0 and n.value == 0
+    assert L.mc_linear_q4_workspace_bytes(17, 256, C.byref(n)) == 0 and n.value == 2 * 16 * 256 * 2
+    refused(lib, L.mc_linear_q4_workspace_bytes(65, 256, C.byref(n)), "bad arguments")
     refused(lib, call(w(), M=-1), "at most 64")
     refused(lib, call(w(), ldx=252), "rows of x")
     refused(lib, call(w(), ldx=248), "rows of x")
@@ -95,7 +101,7 @@ def test_bad_logits_calls(lib):
     refused(lib, call(ld=7), "rows overlap")
     refused(lib, call(prompt_ids=4096, prompt_cols=-1), "negative")
     refused(lib, call(bias_ids=4096, bias=0, n_bias=2), "biases")
-    refused(lib, call(bias_ids=4096, bias=4096, n_bias=4097), "biases")
+    refused(lib, call(bias_ids=4096, bias=4096, n_bias=1025), "biases")
     assert call(M=0) == 0
 
 
