@@ -1135,10 +1135,14 @@ class MultimodalLlamaForCausalLM:
         prompt followed by the new ids, rows that hit EOS are padded with pad_token_id (transformers greedy_search / sample).
         do_sample=True applies transformers 4.31's warpers in their order (temperature, top_k - GenerationConfig default 50, pass
         top_k=0 to disable - then top_p) and draws with a Philox stream keyed by `seed` (kwarg; default: drawn from torch's global
-        generator, so torch.manual_seed makes runs repeatable).  num_beams > 1: beam search (_beam_search; kwargs length_penalty, early_stopping)."""
+        generator, so torch.manual_seed makes runs repeatable).  num_beams > 1: beam search (_beam_search; kwargs length_penalty, early_stopping).
+        repetition_penalty (over the text prompt and the generated ids: RepetitionPenaltyLogitsProcessor), presence_penalty, frequency_penalty
+        (generated ids) and logit_bias ({token id: bias}) change the logits before either rule (ops.logits_process), one launch sequence per token;
+        return_step_logits then returns the processed ones."""
+        penalties = _logits_options(kw, self.config.vocab_size)
         if num_beams not in (None, 1):
-            if do_sample or kw.get("streamer") is not None or kw.get("stopping_criteria") or kw.get("forced_ids") is not None or return_step_logits:
-                raise NotImplementedError("beam search runs greedy-scored, without streamer / stopping criteria / step logits")
+            if do_sample or kw.get("streamer") is not None or kw.get("stopping_criteria") or kw.get("forced_ids") is not None or return_step_logits or penalties:
+                raise NotImplementedError("beam search runs greedy-scored, without streamer / stopping criteria / step logits / penalties")
             return self._beam_search(input_ids, modal_inputs or {}, attention_mask, int(num_beams), max_new_tokens,
                                      float(kw.pop("length_penalty", 1.0)), bool(kw.pop("early_stopping", False)), ignore_eos)
         sampling = None
@@ -1186,7 +1190,7 @@ class MultimodalLlamaForCausalLM:
         feats, _ = self.encode_modal_inputs(modal_inputs, self.prefix_tokens, self.suffix_tokens)
         e1 = mark()
         plan = self._plan(input_ids, attention_mask, None, modal_inputs, feats)
-        st = self._prefill(plan, feats, max_new_tokens, want_logits=return_step_logits or sampling is not None, slot=slot)
+        st = self._prefill(plan, feats, max_new_tokens, want_logits=return_step_logits or sampling is not None or penalties is not None, slot=slot)
         st["mask_in_decode"] = mask_in_decode
         e2 = mark()
         if prefill_done is not None:
@@ -1200,7 +1204,18 @@ class MultimodalLlamaForCausalLM:
                 self._cache[("out_ids", slot, B, max_new_tokens)] = out
             else:
                 out.zero_()
-            if sampling is not None:                                  # first token: same rule, RNG counter -1 (decode steps count from 0)
+            if penalties is not None:
+                pen = penalties.tensors(B, self.device)
+                prompt = input_ids.to(self.device, torch.int64).contiguous()
+
+                def choose(logits, s_):                              # token s_ + 1 from the logits after s_ + 1 generated tokens (s_ = -1: the first)
+                    lg = ops.logits_process(logits, prompt_ids=prompt, output_ids=out[:, :s_ + 1] if s_ >= 0 else None, **pen)
+                    ids = ops.argmax(lg) if sampling is None else ops.sample_step(lg, sampling[0], sampling[1], sampling[2], seed=sampling[3], step=s_)
+                    st["next_ids"].copy_(ids)
+                    out[:, s_ + 1] = ids
+                    return lg
+                st["logits"] = choose(st["logits"], -1)
+            elif sampling is not None:                                # first token: same rule, RNG counter -1 (decode steps count from 0)
                 st["next_ids"].copy_(ops.sample_step(st["logits"], sampling[0], sampling[1], sampling[2], seed=sampling[3], step=-1))
                 st["sampling"] = sampling
             out[:, 0] = st["next_ids"]
@@ -1228,8 +1243,8 @@ class MultimodalLlamaForCausalLM:
                 streamer.put(input_ids.cpu())
             halted = hooks(1) if per_token else False
             if forced is not None:
-                if sampling is not None or per_token or not ignore_eos:
-                    raise ValueError("forced_ids is a greedy, ignore_eos=True, hook-free mode")
+                if sampling is not None or per_token or not ignore_eos or penalties is not None:
+                    raise ValueError("forced_ids is a greedy, ignore_eos=True, hook-free mode without penalties")
                 forced = forced.to(self.device, torch.int64)
                 if forced.numel() and (int(forced.min()) < 0 or int(forced.max()) >= self.model.embed_tokens.shape[0]):
                     raise IndexError(f"forced_ids holds an id outside the embedding table of {self.model.embed_tokens.shape[0]} rows")
@@ -1238,6 +1253,16 @@ class MultimodalLlamaForCausalLM:
                     lg = self._decode(st, 1, out[:, 1:], s_, want_logits=return_step_logits)
                     if return_step_logits:
                         step_logits.append(lg)
+            elif penalties is not None:
+                for s_ in range(max_new_tokens - 1 if not halted else 0):
+                    # (the step's own choice - an arg-max of the raw logits - is replaced; with a column of out to write it to)
+                    lg = choose(self._decode(st, 1, out[:, 1:], s_, want_logits=True)[0], s_)
+                    if return_step_logits:
+                        step_logits.append(lg[None])
+                    if per_token and hooks(2 + s_):
+                        break
+                    if not ignore_eos and s_ % 16 == 15 and bool(((out[:, :2 + s_] == eos).any(dim=1)).all()):      # host sync once in 16 tokens
+                        break
             elif max_new_tokens > 1 and not halted:
                 if ignore_eos and not per_token:
                     lg = self._decode(st, max_new_tokens - 1, out[:, 1:], 0, want_logits=return_step_logits)
@@ -1420,6 +1445,39 @@ class MultimodalLlamaForCausalLM:
 
 # alias kept by the reference's package __init__ (model/__init__.py:1-3); the legacy single-image class is out of scope
 LlavaLlamaForCausalLM = MultimodalLlamaForCausalLM
+
+
+class _LogitsOptions:
+    """generate()'s penalties and biases, checked: tensors(B) are the arguments of ops.logits_process that do not change from step to step."""
+
+    def __init__(self, repetition, presence, frequency, bias):
+        self.repetition, self.presence, self.frequency, self.bias = repetition, presence, frequency, bias
+
+    def tensors(self, B, device):
+        t = lambda v: None if v is None else torch.full((B,), v, dtype=torch.float32, device=device)
+        ids = val = None
+        if self.bias:
+            ids = torch.tensor(list(self.bias), dtype=torch.int32, device=device).expand(B, -1).contiguous()
+            val = torch.tensor(list(self.bias.values()), dtype=torch.float32, device=device).expand(B, -1).contiguous()
+        return dict(repetition_penalty=t(self.repetition), presence_penalty=t(self.presence), frequency_penalty=t(self.frequency), bias_ids=ids, bias=val)
+
+
+def _logits_options(kw, vocab_size):
+    """Takes repetition_penalty, presence_penalty, frequency_penalty and logit_bias out of generate()'s keywords -> _LogitsOptions, or None where none of them
+    changes anything."""
+    rep, pres, freq, bias = (kw.pop(n, None) for n in ("repetition_penalty", "presence_penalty", "frequency_penalty", "logit_bias"))
+    if rep is not None and not (float(rep) > 0 and math.isfinite(rep)):                     # logits_process.py RepetitionPenaltyLogitsProcessor
+        raise ValueError(f"`penalty` has to be a strictly positive float, but is {rep}")
+    for n, v in (("presence_penalty", pres), ("frequency_penalty", freq)):
+        if v is not None and not math.isfinite(v):
+            raise ValueError(f"`{n}` has to be a finite float, but is {v}")
+    bias = {int(t): float(v) for t, v in (bias or {}).items()}
+    if len(bias) > 1024:
+        raise ValueError(f"`logit_bias` holds {len(bias)} tokens, at most 1024 are supported")
+    if any(not 0 <= t < vocab_size or math.isnan(v) for t, v in bias.items()):
+        raise ValueError("`logit_bias` names a token outside the vocabulary or holds a NaN")
+    rep, pres, freq = (None if v is None or float(v) == off else float(v) for v, off in ((rep, 1.0), (pres, 0.0), (freq, 0.0)))
+    return _LogitsOptions(rep, pres, freq, bias) if rep is not None or pres is not None or freq is not None or bias else None
 
 
 def _past_len(pkv):

@@ -633,10 +633,9 @@ _F32, _I32, _I64, _U8 = torch.float32, torch.int32, torch.int64, torch.uint8
 
 
 def _call(name, index, *args):
-    L = _lib.lib()
-    fn = _fns.get((L, name))
-    if fn is None:
-        fn = _fns[(L, name)] = getattr(L, name)
+    fn = _fns.get(name)
+    if fn is None:                                          # (one library per process: _lib.set_storage_dtype)
+        fn = _fns[name] = getattr(_lib.lib(), name)
     if index == torch.cuda.current_device():
         rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
     else:
@@ -900,19 +899,31 @@ def logits_process(logits, prompt_ids=None, prompt_lens=None, output_ids=None, o
         po, ldo = out.data_ptr(), V
     else:
         po, ldo = _arg(out, "out", index, _F32, (M, V)), out.stride(0)
-    hist = []
-    for name, ids, lens in (("prompt", prompt_ids, prompt_lens), ("output", output_ids, output_lens)):
-        if ids is None:
-            if lens is not None:
-                raise ValueError(f"{name}_lens without {name}_ids")
-            hist += (0, 0, 0, 0)
-            continue
-        if ids.dim() != 2:
-            raise ValueError(f"{name}_ids must be 2-D [M, n]")
-        n = ids.shape[1]
-        hist += (_arg(ids, name + "_ids", index, _I64, (M, n)), ids.stride(0), 0 if lens is None else _arg(lens, name + "_lens", index, _I32, (M,)), n)
-    pen = [0 if t is None else _arg(t, n, index, _F32, (M,)) for t, n in (
-        (repetition_penalty, "repetition_penalty"), (presence_penalty, "presence_penalty"), (frequency_penalty, "frequency_penalty"))]
+    pp = ldp = ppl = np_ = pq = ldq = pql = nq = p1 = p2 = p3 = 0
+    if prompt_ids is not None:
+        if prompt_ids.dim() != 2:
+            raise ValueError("prompt_ids must be 2-D [M, n]")
+        np_, ldp = prompt_ids.shape[1], prompt_ids.stride(0)
+        pp = _arg(prompt_ids, "prompt_ids", index, _I64, (M, np_))
+        if prompt_lens is not None:
+            ppl = _arg(prompt_lens, "prompt_lens", index, _I32, (M,))
+    elif prompt_lens is not None:
+        raise ValueError("prompt_lens without prompt_ids")
+    if output_ids is not None:
+        if output_ids.dim() != 2:
+            raise ValueError("output_ids must be 2-D [M, n]")
+        nq, ldq = output_ids.shape[1], output_ids.stride(0)
+        pq = _arg(output_ids, "output_ids", index, _I64, (M, nq))
+        if output_lens is not None:
+            pql = _arg(output_lens, "output_lens", index, _I32, (M,))
+    elif output_lens is not None:
+        raise ValueError("output_lens without output_ids")
+    if repetition_penalty is not None:
+        p1 = _arg(repetition_penalty, "repetition_penalty", index, _F32, (M,))
+    if presence_penalty is not None:
+        p2 = _arg(presence_penalty, "presence_penalty", index, _F32, (M,))
+    if frequency_penalty is not None:
+        p3 = _arg(frequency_penalty, "frequency_penalty", index, _F32, (M,))
     pb = pv = ldb = nb = pa = lda = 0
     if (bias_ids is None) != (bias is None):
         raise ValueError("bias_ids and bias go together")
@@ -926,5 +937,5 @@ def logits_process(logits, prompt_ids=None, prompt_lens=None, output_ids=None, o
     if allowed is not None:
         pa, lda = _arg(allowed, "allowed", index, _I32, (M, (V + 31) // 32)), allowed.stride(0)
     if M and V:
-        _call("mc_logits_process_f32", index, _lib.LogitsArgsC(pl, logits.stride(0), po, ldo, M, V, *hist, *pen, pb, pv, ldb, nb, pa, lda))
+        _call("mc_logits_process_f32", index, _lib.LogitsArgsC(pl, logits.stride(0), po, ldo, M, V, pp, ldp, ppl, np_, pq, ldq, pql, nq, p1, p2, p3, pb, pv, ldb, nb, pa, lda))
     return out
