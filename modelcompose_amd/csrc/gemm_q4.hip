@@ -88,7 +88,7 @@ __global__ __launch_bounds__(W * 64) void linear_q4_kernel(Q4Params p) {
     auto load_w = [&](int u, int i) {
         const int k = (first + min(i, count - 1)) * kQ4Block, last = ((p.K - k) >> 5) - 1;      // last: index of the last piece of 32 columns
 #pragma unroll
-        for (int r = 0; r < R; ++r) wq[u][r] = __builtin_nontemporal_load((const u32x4*)(wrow[r] + (k >> 1) + 16 * min(g, last)));
+        for (int r = 0; r < R; ++r) wq[u][r] = *(const u32x4*)(wrow[r] + (k >> 1) + 16 * min(g, last));      // (cached: half a line now, half with the next block)
     };
     // scales and zero points of blocks 8 t .. 8 t + 7 of the chunk: quarter g holds those of blocks 8 t + 2 g and the next, 2 NG of them
     constexpr int ZW = NG == 4 ? 2 : 1;
@@ -157,7 +157,7 @@ __global__ __launch_bounds__(W * 64) void linear_q4_kernel(Q4Params p) {
             }
             if (ZP) {
                 zv[r] = (uint32_t)__builtin_amdgcn_ds_bpermute(from, (int)o.z[r][NG == 4 ? odd : 0]);
-                if (NG < 4 && odd) zv[r] >>= 8 * NG;
+                if constexpr (NG < 4) { if (odd) zv[r] >>= 8 * NG; }
             }
         }
 #pragma unroll
