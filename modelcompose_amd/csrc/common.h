@@ -116,6 +116,14 @@ __device__ __forceinline__ float attn_dropout_one(const AttnDropout& d, int64_t 
     return m[key & 3];
 }
 
+// a * b rounded to fp32 on its own: the compiler may not fuse it with the addition behind it.  Where a sum of products is not pinned like this (or by
+// fmaf), its last bit follows whether the compiler happens to pack pairs of floats.
+__device__ __forceinline__ float product_rounded(float a, float b) {
+    float q = a * b;
+    asm("" : "+v"(q));
+    return q;
+}
+
 __device__ __forceinline__ float wave_sum(float v) {
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);

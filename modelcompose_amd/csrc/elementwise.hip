@@ -34,14 +34,14 @@ __global__ __launch_bounds__(256) void norm_kernel(const bf16_t* __restrict__ x,
                 const float f = (float)t[j];
                 v[it][j] = f;
                 s1 += f;
-                s2 += f * f;
+                s2 += product_rounded(f, f);
             }
         }
     }
     for (int i = 1024 + threadIdx.x; i < nv; i += 256) {
         const bf16x8 t = *(const bf16x8*)(xr + i * 8);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) { const float f = (float)t[j]; s1 += f; s2 += f * f; }
+        for (int j = 0; j < 8; ++j) { const float f = (float)t[j]; s1 += f; s2 += product_rounded(f, f); }
     }
     float mean = 0.f, rstd;
     if (RMS) {
@@ -57,13 +57,13 @@ __global__ __launch_bounds__(256) void norm_kernel(const bf16_t* __restrict__ x,
             const int i = it * 256 + threadIdx.x;
             if (i < nv) {
 #pragma unroll
-                for (int j = 0; j < 8; ++j) { const float d = v[it][j] - mean; sv += d * d; }
+                for (int j = 0; j < 8; ++j) { const float d = v[it][j] - mean; sv += product_rounded(d, d); }
             }
         }
         for (int i = 1024 + threadIdx.x; i < nv; i += 256) {
             const bf16x8 t = *(const bf16x8*)(xr + i * 8);
 #pragma unroll
-            for (int j = 0; j < 8; ++j) { const float d = (float)t[j] - mean; sv += d * d; }
+            for (int j = 0; j < 8; ++j) { const float d = (float)t[j] - mean; sv += product_rounded(d, d); }
         }
         sv = block_sum(sv, red);
         rstd = rsqrtf(sv / D + eps);
@@ -125,7 +125,7 @@ __global__ __launch_bounds__(256) void norm_rows_kernel(const bf16_t* __restrict
                 const float f = (float)t[j];
                 v[it][j] = f;
                 s1 += f;
-                s2 += f * f;
+                s2 += product_rounded(f, f);
             }
         }
     }
@@ -139,7 +139,7 @@ __global__ __launch_bounds__(256) void norm_rows_kernel(const bf16_t* __restrict
         for (int it = 0; it < 4; ++it) {
             if (it * 64 + lane < nv) {
 #pragma unroll
-                for (int j = 0; j < 8; ++j) { const float d = v[it][j] - mean; sv += d * d; }
+                for (int j = 0; j < 8; ++j) { const float d = v[it][j] - mean; sv += product_rounded(d, d); }
             }
         }
         rstd = rsqrtf(wave_sum(sv) / D + eps);
@@ -221,7 +221,7 @@ __global__ __launch_bounds__(256) void add_norm_rows_kernel(const bf16_t* __rest
     for (int it = 0; it < 4; ++it) {
         if (it * 64 + lane < nv) {
 #pragma unroll
-            for (int j = 0; j < 8; ++j) { const float d = v[it][j] - mean; sv += d * d; }
+            for (int j = 0; j < 8; ++j) { const float d = v[it][j] - mean; sv += product_rounded(d, d); }
         }
     }
     const float rstd = rsqrtf(wave_sum(sv) / D + eps);
@@ -261,7 +261,7 @@ __global__ __launch_bounds__(256) void rms_scale_kernel(const bf16_t* __restrict
     for (int i = threadIdx.x; i < (D >> 3); i += 256) {
         const bf16x8 t = *(const bf16x8*)(xr + i * 8);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) { const float f = (float)t[j]; s2 += f * f; }
+        for (int j = 0; j < 8; ++j) { const float f = (float)t[j]; s2 += product_rounded(f, f); }
     }
     s2 = block_sum(s2, red);
     if (threadIdx.x == 0) rs[row] = rsqrtf(s2 / D + eps);

@@ -71,8 +71,8 @@ __global__ __launch_bounds__(256) void layernorm_bwd_kernel(const bf16_t* __rest
     const float rstd = rsqrtf(block_sum(sv, red) / D + eps);
     float a = 0.f, b = 0.f;
     for (int i = threadIdx.x; i < D; i += 256) {
-        const float xh = ((float)xr[i] - mean) * rstd, dg = (float)dyr[i] * (float)g[i];
-        a += dg; b += dg * xh;
+        const float xh = ((float)xr[i] - mean) * rstd, dg = product_rounded((float)dyr[i], (float)g[i]);
+        a += dg; b += product_rounded(dg, xh);
     }
     a = block_sum(a, red) / D;
     b = block_sum(b, red) / D;
