@@ -305,7 +305,8 @@ void q4_launch(const Q4Params& p, hipStream_t s) {
 // ---- weights ----------------------------------------------------------------------------------------------------------------------
 // Codes, scales and zero points of a 16-bit weight: a group of g elements on g / 8 lanes.  Symmetric: scale = st(amax / 7), code = rne(w / scale) + 8;
 // with zero points: scale = st((max - min) / 15) over the range widened to hold 0, zero = rne(-min / scale), code = rne(w / scale) + zero; codes
-// clamped to 0..15.  Codes come from the scale as it is stored (st = rounded to 16 bits), so the products the kernels form are the nearest ones.
+// clamped to 0..15.  Codes come from the scale as it is stored (st = rounded to 16 bits), so the products the kernels form are the nearest ones.  A group that holds
+// an infinity or NaN gets the scale NaN: what it multiplies becomes NaN.
 __global__ __launch_bounds__(256) void quantize_q4_kernel(const bf16_t* w, int64_t ldw, uint8_t* codes, bf16_t* scales, uint8_t* zeros, int N, int K, int gshift) {
     const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, per = K / 8;      // K / 8 lanes per row; groups never straddle waves (group <= 128: 16 lanes)
     const bool in = i < N * per;
@@ -313,10 +314,11 @@ __global__ __launch_bounds__(256) void quantize_q4_kernel(const bf16_t* w, int64
     bf16x8 v = {};
     if (in) v = *(const bf16x8*)(w + n * ldw + k);
     float lo = 0.f, hi = 0.f;
+    int odd = 0;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) { lo = fminf(lo, (float)v[j]); hi = fmaxf(hi, (float)v[j]); }
-    for (int o = (1 << gshift) / 16; o > 0; o >>= 1) { lo = fminf(lo, __shfl_xor(lo, o, 64)); hi = fmaxf(hi, __shfl_xor(hi, o, 64)); }
-    const float s = (float)(bf16_t)(zeros ? (hi - lo) / 15.f : fmaxf(hi, -lo) / 7.f);
+    for (int j = 0; j < 8; ++j) { const float f = (float)v[j]; lo = fminf(lo, f); hi = fmaxf(hi, f); odd |= !(fabsf(f) < INFINITY); }
+    for (int o = (1 << gshift) / 16; o > 0; o >>= 1) { lo = fminf(lo, __shfl_xor(lo, o, 64)); hi = fmaxf(hi, __shfl_xor(hi, o, 64)); odd |= __shfl_xor(odd, o, 64); }
+    const float s = odd ? __uint_as_float(0x7fc00000u) : (float)(bf16_t)(zeros ? (hi - lo) / 15.f : fmaxf(hi, -lo) / 7.f);
     const float z = zeros ? fminf(fmaxf(s > 0.f ? rintf(-lo / s) : 0.f, 0.f), 15.f) : 8.f;
     uint32_t out = 0;
 #pragma unroll
@@ -356,7 +358,7 @@ int group_shift(int group) { return group == 32 ? 5 : group == 64 ? 6 : group ==
 int check_weight(const mc_q4_weight* w, const char* who) {
     MC_CHECK_ARG(w && w->codes && w->scales, "%s: null weight", who);
     MC_CHECK_ARG(group_shift(w->group) >= 0, "%s: group %d not supported (32, 64 or 128)", who, w->group);
-    MC_CHECK_ARG(w->N > 0 && w->K > 0 && w->K % w->group == 0, "%s: N = %d, K = %d must be positive and K a multiple of the group %d", who, w->N, w->K, w->group);
+    MC_CHECK_ARG(w->N > 0 && w->N <= (1 << 30) && w->K > 0 && w->K <= (1 << 22) && w->K % w->group == 0, "%s: N = %d, K = %d must be positive, K a multiple of the group %d and at most 2^22", who, w->N, w->K, w->group);
     MC_CHECK_ARG((uintptr_t)w->codes % 16 == 0 && w->ldc % 16 == 0 && w->ldc >= w->K / 2, "%s: rows of codes must be 16-byte aligned", who);
     MC_CHECK_ARG((uintptr_t)w->scales % 2 == 0 && w->lds >= w->K / w->group && (!w->zeros || w->ldz >= w->K / w->group), "%s: bad scales or zeros", who);
     return 0;
@@ -391,14 +393,14 @@ extern "C" int mc_linear_q4_bf16(const void* x, int64_t ldx, const mc_q4_weight*
 }
 
 extern "C" int mc_linear_q4_workspace_bytes(int M, int K, int64_t* bytes) {
-    MC_CHECK_ARG(bytes && M >= 0 && M <= 64 && K > 0, "mc_linear_q4_workspace_bytes: bad arguments");
+    MC_CHECK_ARG(bytes && M >= 0 && M <= 64 && K > 0 && K <= (1 << 22), "mc_linear_q4_workspace_bytes: bad arguments");
     *bytes = M > 16 ? (int64_t)((M + 15) / 16) * 16 * K * 2 : 0;
     return 0;
 }
 
 extern "C" int mc_quantize_q4_bf16(const void* w, int64_t ldw, void* codes, void* scales, void* zeros, int N, int K, int group, void* stream) {
     MC_CHECK_ARG(w && codes && scales, "mc_quantize_q4_bf16: null pointer");
-    MC_CHECK_ARG(group_shift(group) >= 0 && N > 0 && K > 0 && K % group == 0, "mc_quantize_q4_bf16: N = %d, K = %d, group %d (32, 64 or 128, dividing K)", N, K, group);
+    MC_CHECK_ARG(group_shift(group) >= 0 && N > 0 && N <= (1 << 30) && K > 0 && K <= (1 << 22) && K % group == 0, "mc_quantize_q4_bf16: N = %d, K = %d, group %d (32, 64 or 128, dividing K)", N, K, group);
     MC_CHECK_ARG((uintptr_t)w % 16 == 0 && ldw % 8 == 0 && ldw >= K && (uintptr_t)codes % 16 == 0, "mc_quantize_q4_bf16: rows must be 16-byte aligned");
     const int64_t blocks = ((int64_t)N * (K / 8) + 255) / 256;
     MC_CHECK_ARG(blocks < (1LL << 23), "mc_quantize_q4_bf16: %d x %d is too large for one launch", N, K);

@@ -146,8 +146,8 @@ __device__ __forceinline__ int attn8_len(const AttnParams8& p, int b) {
     return max(0, min(n, p.c.S));
 }
 
-// Keys of one partial: a function of the sequence's own length, so that short sequences still spread over many workgroups and long ones are not ground into
-// partials.
+// Keys of one partial: a function of the sequence's own length, so that short sequences still spread over many workgroups (1 x 2809 keys: 13 us with 512, 18 with 1024)
+// and long ones are not ground into partials (8 x 32768 keys: 129 us with 512, 94 with 2048).
 __host__ __device__ inline int attn8_chunk(int n) { return n <= 4096 ? 512 : n <= 16384 ? 1024 : 2048; }
 typedef float f32x4_u __attribute__((ext_vector_type(4), aligned(4)));
 typedef uint32_t u32x2_u __attribute__((ext_vector_type(2), aligned(1)));
@@ -245,10 +245,14 @@ __device__ __forceinline__ void attn8_append(const AttnParams8& p, int b, int hk
 // c & 7 - exactly the layout in which the next product O^T = V^T P^T wants its B operand, so the probabilities never leave the lane.  They
 // enter that product as bfloat16, a high part in columns 0 .. 7 and the remainder in columns 8 .. 15 (w = p * v_scale = hi + lo to 2^-17): the second half of
 // the columns carries the accuracy that 8 significant bits lack, at no instruction.  (bfloat16 also in the half-precision build: w has a wide range.)
-// V^T's operand needs 8 keys of one element per lane: 8 loads of D / 16 bytes per lane (whole 128-byte rows per quarter wave), the bytes paired by v_perm.
+// V^T's operand needs 8 keys of one element per lane: the bytes of two keys' rows are paired by v_perm.
 //
-// A workgroup of 4 waves takes chunks of 512 keys, blockIdx.y, + gridDim.y, ..; wave w the 32-key tiles w, w + 4, .. of a chunk, from a fresh (m, l, acc); the
+// A workgroup of 4 waves takes chunks (attn8_chunk keys) blockIdx.y, + gridDim.y, ..; wave w the 32-key tiles w, w + 4, .. of a chunk, from a fresh (m, l, acc); the
 // waves are joined through LDS in wave order, the chunks by attn8_join in chunk order.  Which workgroup takes which chunk changes no bit.
+//
+// HBM-bound with many sequences: 48 x 2809 keys, 32 heads, D = 128 144 us = 5.8 TB/s (a kernel on the vector units, one head per workgroup: 157; the same loads
+// without the arithmetic: 138); 8 x 32768 keys, 32 heads over 8 92 us = 4.3 TB/s (757).  Latency-bound with few: 1 x 2809 keys 13 us, 3.8 of them the join.
+// Three waves per SIMD at D = 128 (168 registers): with two 162 us, with four the tile spills (229).
 template <int D, int FMT, bool KM>
 __global__ __launch_bounds__(256, D == 128 ? 3 : 4) void attn_decode8_kernel(AttnParams8 p) {
     // (a score and the maximum taken from it have to be the same number: fused into the difference, the score's product would not be rounded, and at 1e30 the
@@ -575,7 +579,7 @@ int check_rope(const void* qkv, int64_t ld, const float* cos_table, const float*
     return 0;
 }
 
-// enough workgroups to fill the chip several times over, while there are chunks to hand out
+// 4096 workgroups fill the chip five times over, while there are chunks to hand out (48 x 2809 keys: 160 us with 4608 workgroups, 167 with 1536, 169 with 9216)
 int attn8_launch(AttnParams8& p, const mc_kv8_cache* c, hipStream_t s, const char* who) {
     const int chunks = attn8_max_parts(c->S);
     p.G = p.H / c->Hkv;
@@ -583,7 +587,8 @@ int attn8_launch(AttnParams8& p, const mc_kv8_cache* c, hipStream_t s, const cha
     p.ws_chunks = chunks;
     const int64_t wgs = (int64_t)c->B * c->Hkv * p.groups;
     MC_CHECK_ARG(wgs < (1LL << 23) && (int64_t)c->B * p.H < (1LL << 23), "%s: B * H = %lld is too large for one launch", who, (long long)c->B * p.H);
-    // up to two chunks: one workgroup takes both and joins them itself, the second launch costs more (5 x 517 keys: 8.5 against 10.2 us)
+    // up to two chunks: one workgroup takes both and joins them itself.  Launched one call at a time the second launch costs more than it saves (5 x 517 keys: 14.8
+    // against 17.4 us a call; replayed from a graph 12.2 against 10.1)
     const int want = (int)((4096 + wgs - 1) / wgs), split = chunks <= 2 ? 1 : want < chunks ? want : chunks;
     p.self_combine = split == 1;
     const dim3 grid((unsigned)wgs, split);

@@ -357,6 +357,50 @@ def test_a_row_does_not_depend_on_its_batch_or_the_cache_size():
     assert torch.equal(ops.attn_decode8(q[7:8], sub), whole[7:8])
 
 
+@pytest.mark.parametrize("lens", [(4096, 4097, 4100, 33), (16384, 16385, 16390, 4095), (20000, 5, 16383, 18433)])
+def test_lengths_around_a_change_of_the_chunk(lens):
+    from modelcompose_amd import ops
+    g = _gen(lens[0])
+    S, D = max(lens) + 70, 64
+    cache, host = make_cache(g, len(lens), 1, S, D, "int8")
+    q = _rand(g, len(lens), 3, D) * 2
+    n = torch.tensor(lens, dtype=torch.int32)
+    got = ops.attn_decode8(q.cuda(), cache, kv_lens=n.cuda())
+    near(got.view(-1, 3, D), *attend(q.double(), host, lens, 1 / math.sqrt(D)))
+    for b in range(len(lens)):                                                          # alone, in a cache of its own length
+        one = ops.Kv8Cache(*(t[b:b + 1, :, :lens[b]] for t in (cache.k, cache.k_scale, cache.v, cache.v_scale)))
+        assert torch.equal(ops.attn_decode8(q[b:b + 1].cuda(), one)[0], got[b])
+
+
+def test_more_partials_than_a_batch_of_the_join():
+    """600 000 keys: 293 partials of 2048 keys."""
+    from modelcompose_amd import ops
+    g = _gen(77)
+    S, D = 600_000, 64
+    cache, host = make_cache(g, 1, 1, S, D, "int8")
+    host[1][0, 0, 500_000:500_064] *= 6                                                    # some weight late, in the second batch of partials
+    cache.k_scale.copy_(host[1])
+    q = _rand(g, 1, 2, D)
+    near(ops.attn_decode8(q.cuda(), cache).view(1, 2, D), *attend(q.double(), host, [S], 1 / math.sqrt(D)))
+
+
+def test_workgroups_that_take_several_chunks():
+    """So many sequences that a workgroup takes every other chunk: the same bits as one sequence at a time, whose workgroups take one."""
+    from modelcompose_amd import ops
+    g = _gen(78)
+    B, H, S, D = 48, 48, 1800, 64
+    cache = ops.kv8_cache(B, H, S, D)
+    for t, s in ((cache.k, cache.k_scale), (cache.v, cache.v_scale)):
+        t.view(torch.uint8).copy_(torch.randint(0, 120, t.shape, dtype=torch.uint8, device="cuda"))
+        s.uniform_(0.001, 0.01)
+    lens = torch.randint(1, S + 1, (B,), generator=g).int().cuda()
+    q = _rand(g, B, H, D).cuda()
+    whole = ops.attn_decode8(q, cache, kv_lens=lens)
+    for b in (0, 13, 47):
+        one = ops.Kv8Cache(*(t[b:b + 1] for t in (cache.k, cache.k_scale, cache.v, cache.v_scale)))
+        assert torch.equal(ops.attn_decode8(q[b:b + 1], one, kv_lens=lens[b:b + 1])[0], whole[b])
+
+
 def test_offsets_past_32_bits():
     """A cache of more than 2^31 bytes: written, read and attended at its far end."""
     from modelcompose_amd import ops
@@ -376,7 +420,11 @@ def test_offsets_past_32_bits():
     keep = torch.zeros(1, S, dtype=torch.uint8, device="cuda")
     keep[0, S - 1] = 1
     out = ops.attn_decode8(x[:, :Hkv * D].view(1, Hkv, D).cuda(), cache, key_valid=keep)
-    assert torch.equal(out.cpu().view(Hkv, D), (c.float() * s[:, None]).to(_st()))
+    # one key: its weight is 1, and w = 1 * v_scale enters the product as hi + lo, each rounded to bfloat16.  For w in [1, 2) (any binade alike) the rest
+    # w - hi is at most 2^-8, and below 2^-8 a bfloat16 step is at most 2^-16: lo is off by 2^-17 at most.  The code is exact, the two products are added
+    # in fp32 (2^-23) and the division by the sum 1 is exact; the rounding to the storage type adds half a step.
+    ref = c.double() * s.double()[:, None]
+    assert ((out.cpu().view(Hkv, D).double() - ref).abs() <= ref.abs() * (torch.finfo(_st()).eps / 2 + 2 ** -17 + 2 ** -22)).all()
     _, vr = ops.kv8_read(cache)
     assert torch.equal(vr[0, :, S - 1].cpu(), (c.float() * s[:, None]).to(_st())) and int((vr != 0).sum()) == int((vr[0, :, S - 1] != 0).sum())
 
@@ -453,6 +501,17 @@ def test_quantize_and_dequantize_q4(N, K, group, symmetric):
     wt.copy_(w)
     q2 = ops.quantize_q4(wt, group, symmetric)
     assert torch.equal(q2.codes, q.codes) and torch.equal(q2.scales, q.scales)
+
+
+@pytest.mark.parametrize("symmetric", [True, False])
+def test_quantize_q4_of_non_finite_weights(symmetric):
+    from modelcompose_amd import ops
+    w = torch.ones(4, 128).to(_st())
+    w[1, 40], w[2, 70], w[3, 127] = math.inf, math.nan, -math.inf
+    q = ops.quantize_q4(w.cuda(), 32, symmetric)
+    assert torch.equal(torch.isnan(q.scales.cpu()), torch.tensor([[0, 0, 0, 0], [0, 1, 0, 0], [0, 0, 1, 0], [0, 0, 0, 1]]).bool())
+    y = ops.linear_q4(torch.ones(1, 128, dtype=_st(), device="cuda"), q)
+    assert torch.isnan(y[0, 1:]).all() and torch.isfinite(y[0, 0])
 
 
 # ---- logits ----------------------------------------------------------------------------------------------------------------------------
