@@ -393,7 +393,7 @@ int mc_sample_step_f32(const float* logits, int64_t ld, int64_t* next_ids, int64
  * beam_search, forwarded by eval/model_multimodal_qa_loader.py:94-102) */
 int mc_log_softmax_f32(const float* logits, int64_t ld, float* out, int64_t ldo, int M, int N, void* stream);
 
-/* Logits processor (csrc/logits.hip), before mc_argmax_f32 / mc_sample_step_f32; out may be logits (in place).  For row m, token t:
+/* Logits processor (csrc/logits.hip), before mc_argmax_f32 / mc_sample_step_f32; out is logits (in place) or does not overlap it.  For row m, token t:
  *   seen = t among the prompt or output ids, c = its number among the output ids
  *   l = seen ? (l > 0 ? l / repetition[m] : l * repetition[m]) : l;   l -= frequency[m] * c + presence[m] * (c > 0);
  *   l += sum of bias[m][i] over bias_ids[m][i] == t;   l = -inf unless bit t & 31 of allowed[m][t >> 5] is set.
@@ -417,7 +417,8 @@ typedef struct mc_q4_weight {
     int N, K, group;
 } mc_q4_weight;
 /* out[M, N] = x[M, K] W^T (+ bias) (+ residual): at most 64 rows; out 16-bit, or fp32 with out_f32.  Codes are multiplied as exact integers and summed in
- * fp32 per group, then scaled; a row's result does not depend on M. */
+ * fp32 per group, the zero point is taken out as zero * sum(x), then scaled: an infinity in a row of x gives NaN.  A row's result does not depend on M.
+ * out may be residual, but may not overlap x. */
 int mc_linear_q4_bf16(const void* x, int64_t ldx, const mc_q4_weight* w, const void* bias, const void* residual, int64_t ldr, void* out, int64_t ldo,
                       int M, int out_f32, void* workspace, void* stream);
 /* scratch of that call (0 up to 16 rows: workspace may be NULL), 16-byte aligned */
@@ -446,7 +447,7 @@ int mc_rope_kv8(const void* qkv, int64_t ld, const int32_t* row_b, const int32_t
 /* k_out / v_out [B, Hkv, n, D] 16-bit = code * scale of the first n positions; positions >= kv_lens[b] (NULL: none) are zero rows */
 int mc_kv8_read(const mc_kv8_cache* cache, const int32_t* kv_lens, int n, void* k_out, void* v_out, void* stream);
 /* Decode attention (one query per sequence) over the first kv_lens[b] (clipped to S; NULL: S) keys; key_valid as in mc_attn_mask.  A sequence without a
- * key gives a zero row.  A row's bits depend neither on B nor on S (chunks of keys at fixed positions, combined in order). */
+ * key gives a zero row.  o may not overlap q, workspace no other call's in flight.  A row's bits depend neither on B nor on S (chunks of keys at fixed positions, combined in order). */
 int mc_attn_decode8_workspace_bytes(int B, int H, int D, int S, int64_t* bytes);
 int mc_attn_decode8(const void* q, int64_t q_sb, int64_t q_sh, const mc_kv8_cache* cache, const int32_t* kv_lens, const void* key_valid,
                     int64_t key_valid_stride, void* o, int64_t o_sb, void* workspace, int H, float scale, void* stream);

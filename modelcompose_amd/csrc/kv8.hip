@@ -586,6 +586,7 @@ int attn8_launch(AttnParams8& p, const mc_kv8_cache* c, hipStream_t s, const cha
     p.groups = (p.G + 7) / 8;
     p.ws_chunks = chunks;
     const int64_t wgs = (int64_t)c->B * c->Hkv * p.groups;
+    MC_CHECK_ARG(c->B == 1 || p.o_sb >= (int64_t)p.H * c->D, "%s: output rows overlap", who);
     MC_CHECK_ARG(wgs < (1LL << 23) && (int64_t)c->B * p.H < (1LL << 23), "%s: B * H = %lld is too large for one launch", who, (long long)c->B * p.H);
     // up to two chunks: one workgroup takes both and joins them itself.  Launched one call at a time the second launch costs more than it saves (5 x 517 keys: 14.8
     // against 17.4 us a call; replayed from a graph 12.2 against 10.1)

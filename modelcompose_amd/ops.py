@@ -724,7 +724,8 @@ def dequantize_q4(w: Q4Weight) -> PackedWeight:
 def linear_q4(x: torch.Tensor, w: Q4Weight, residual: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None, out_f32: bool = False,
               bias: bool = True) -> torch.Tensor:
     """out[M, N] = x W^T (+ bias) (+ residual) for at most 64 rows x [M, K] (the decode step's form of linear(); larger launches: linear(x,
-    dequantize_q4(w)), with x padded to its Kp).  fp32 sums; the codes enter as exact integers.  A row's bits do not depend on M."""
+    dequantize_q4(w)), with x padded to its Kp).  fp32 sums; the codes enter as exact integers, the zero point as zero * sum(x) (an infinity in x gives NaN).
+    A row's bits do not depend on M.  out may be the residual, but may not overlap x."""
     index = _device(x, "x")
     if x.dim() != 2:
         raise ValueError("x must be 2-D [M, K]")
@@ -863,7 +864,7 @@ def _decode8(name, head, cache, H, kv_lens, out, scale, key_valid):
 
 def attn_decode8(q, cache: Kv8Cache, kv_lens=None, out=None, scale=None, key_valid=None):
     """Decode attention over an 8-bit cache: q [B, H, D] (one rotated query per sequence; H a multiple of Hkv), kv_lens int32 [B] (None: every position) ->
-    out [B, H * D].  key_valid uint8 / bool [B, >= S]: 0 = masked.  A sequence without a key gives zeros."""
+    out [B, H * D].  key_valid uint8 / bool [B, >= S]: 0 = masked.  A sequence without a key gives zeros.  out may not overlap q."""
     index = _device(q, "q")
     if q.dim() != 3:
         raise ValueError("q must be [B, H, D]")
@@ -888,7 +889,8 @@ def logits_process(logits, prompt_ids=None, prompt_lens=None, output_ids=None, o
     """Penalties, biases and a token mask on logits [M, V] fp32, before argmax() / sample_step() (out=logits: in place).
     prompt_ids / output_ids int64 [M, n] with optional int32 lengths [M]: the repetition penalty (l / r or l * r) reads both, frequency * count + presence
     only the output ids.  The penalties are fp32 tensors [M]; bias_ids int32 [M, n] with bias fp32 [M, n] (a token may be listed twice: the biases add up);
-    allowed int32 [M, ceil(V / 32)]: bit t & 31 of word t >> 5 clear = -inf.  Ids outside [0, V) are ignored."""
+    allowed int32 [M, ceil(V / 32)]: bit t & 31 of word t >> 5 clear = -inf.  Ids outside [0, V) are ignored.
+    out is logits itself or does not overlap it."""
     index = _device(logits, "logits")
     if logits.dim() != 2:
         raise ValueError("logits must be 2-D [M, V]")

@@ -61,6 +61,13 @@ def test_bad_cache_calls(lib):
     refused(lib, L.mc_attn_decode8_workspace_bytes(0, 1, 128, 1, C.byref(n)), "bad arguments")
 
 
+def test_output_rows_that_overlap(lib):
+    L, c, one = lib.lib(), C.byref(cache_c(lib)), 4096
+    for stride in (0, 511):                                                                # 4 heads of 128: 512
+        refused(lib, L.mc_attn_decode8(one, 512, 128, c, None, None, 0, one, stride, one, 4, 1.0, None), "output rows overlap")
+        refused(lib, L.mc_attn_decode8_rope(one, 1024, one, one, 16, c, one, None, 0, one, stride, one, 4, 1.0, None), "output rows overlap")
+
+
 def test_bad_q4_calls(lib):
     L, one = lib.lib(), 4096
 
