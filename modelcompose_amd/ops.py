@@ -636,7 +636,7 @@ def _call(name, index, *args):
     fn = _fns.get(name)
     if fn is None:                                          # (one library per process: _lib.set_storage_dtype)
         fn = _fns[name] = getattr(_lib.lib(), name)
-    if index == torch.cuda.current_device():
+    if index == torch._C._cuda_getDevice():                 # (a tensor of the device exists: HIP is initialised)
         rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
     else:
         with torch.cuda.device(index):
@@ -736,7 +736,7 @@ def linear_q4(x: torch.Tensor, w: Q4Weight, residual: Optional[torch.Tensor] = N
     if w.index != index:
         raise ValueError(f"the weight is on device {w.index}, x on device {index}")
     if out is None:
-        out = torch.empty((M, N), dtype=dt, device=x.device)
+        out = torch.empty((M, N), dtype=_F32, device=x.device) if out_f32 else x.new_empty((M, N))
         po, ldo = out.data_ptr(), N
     else:
         po, ldo = _arg(out, "out", index, dt, (M, N)), out.stride(0)
@@ -839,11 +839,10 @@ def _decode8_scratch(B, H, D, S):
     return n.value
 
 
-def _decode8(name, head, cache, H, kv_lens, out, scale, key_valid):
+def _decode8(name, head, x, cache, H, kv_lens, out, scale, key_valid):
     """The arguments that attn_decode8 and attn_decode8_rope share, and the call.  The scratch is the caching allocator's: calls in flight on other streams, and
     captured graphs, have their own."""
     B, D, S, index = cache.B, cache.D, cache.S, cache.index
-    dev = cache.k.device
     pl = 0 if kv_lens is None else _arg(kv_lens, "kv_lens", index, _I32, (B,))
     pm = ms = 0
     if key_valid is not None:
@@ -853,11 +852,11 @@ def _decode8(name, head, cache, H, kv_lens, out, scale, key_valid):
             raise ValueError(f"key_valid must be [B, >= {S}], got {tuple(key_valid.shape)}")
         pm, ms = _arg(key_valid, "key_valid", index, _U8, (B, key_valid.shape[1])), key_valid.stride(0)
     if out is None:
-        out = torch.empty((B, H * D), dtype=BF16, device=dev)
+        out = x.new_empty((B, H * D))
         po, so = out.data_ptr(), H * D
     else:
         po, so = _arg(out, "out", index, BF16, (B, H * D)), out.stride(0)
-    ws = torch.empty(_decode8_ws.get((B, H, D, S)) or _decode8_scratch(B, H, D, S), dtype=_U8, device=dev)
+    ws = torch.empty(_decode8_ws.get((B, H, D, S)) or _decode8_scratch(B, H, D, S), dtype=_U8, device=x.device)
     _call(name, index, *head, cache._c, pl, pm, ms, po, so, ws.data_ptr(), H, D ** -0.5 if scale is None else scale)
     return out
 
@@ -872,7 +871,7 @@ def attn_decode8(q, cache: Kv8Cache, kv_lens=None, out=None, scale=None, key_val
     pq = _arg(q, "q", index, BF16, (cache.B, H, cache.D))
     if cache.index != index:
         raise ValueError(f"the cache is on device {cache.index}, q on device {index}")
-    return _decode8("mc_attn_decode8", (pq, q.stride(0) if cache.B > 1 else cache.D, q.stride(1) if H > 1 else cache.D), cache, H, kv_lens, out, scale, key_valid)
+    return _decode8("mc_attn_decode8", (pq, q.stride(0) if cache.B > 1 else cache.D, q.stride(1) if H > 1 else cache.D), q, cache, H, kv_lens, out, scale, key_valid)
 
 
 def attn_decode8_rope(qkv, cos, sin, cache: Kv8Cache, kv_lens, H, out=None, scale=None, key_valid=None):
@@ -881,7 +880,7 @@ def attn_decode8_rope(qkv, cos, sin, cache: Kv8Cache, kv_lens, H, out=None, scal
     if kv_lens is None:
         raise ValueError("kv_lens is needed: it places the new token")
     index, p, ld, pc, ps, n_pos = _rope_args(qkv, cos, sin, cache, H, cache.B)
-    return _decode8("mc_attn_decode8_rope", (p, ld, pc, ps, n_pos), cache, H, kv_lens, out, scale, key_valid)
+    return _decode8("mc_attn_decode8_rope", (p, ld, pc, ps, n_pos), qkv, cache, H, kv_lens, out, scale, key_valid)
 
 
 def logits_process(logits, prompt_ids=None, prompt_lens=None, output_ids=None, output_lens=None, repetition_penalty=None, presence_penalty=None,
@@ -897,7 +896,7 @@ def logits_process(logits, prompt_ids=None, prompt_lens=None, output_ids=None, o
     M, V = logits.shape
     pl = _arg(logits, "logits", index, _F32, (M, V))
     if out is None:
-        out = torch.empty((M, V), dtype=_F32, device=logits.device)
+        out = logits.new_empty((M, V))
         po, ldo = out.data_ptr(), V
     else:
         po, ldo = _arg(out, "out", index, _F32, (M, V)), out.stride(0)
