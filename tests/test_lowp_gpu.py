@@ -471,6 +471,22 @@ def test_linear_q4(M, N, K, group, zeros):
     assert torch.equal(ops.linear_q4(x.cuda(), w, residual=res2, out=res2), y)               # the residual updated in place
 
 
+@pytest.mark.parametrize("M", [3, 16, 20, 40, 61])
+@pytest.mark.parametrize("N,K,group,zeros", [(4100, 96, 32, True), (5001, 1184, 32, False), (8192, 640, 64, True), (4111, 9088, 128, True),       # two blocks of columns per workgroup
+                                             (8193, 32, 32, False), (8240, 1056, 32, True), (9001, 704, 64, False), (8208, 5248, 128, True), (8225, 4736, 64, True)])     # three
+def test_linear_q4_of_many_columns(M, N, K, group, zeros):
+    from modelcompose_amd import ops
+    g = _gen(N * 37 + M)
+    codes, scales, z = random_q4(g, N, K, group, zeros)
+    x = _rand(g, M, K) + 0.25
+    w = ops.Q4Weight(codes.cuda(), scales.cuda(), None if z is None else z.cuda())
+    ref, mag = q4_ref(x, codes, scales, z, group)
+    y = ops.linear_q4(x.cuda(), w, out_f32=True)
+    near(y, ref, (K + 16) * U * mag + 1e-30)
+    assert torch.equal(ops.linear_q4(x[M - 1:].cuda(), w, out_f32=True)[0], y[M - 1])
+    assert torch.equal(ops.linear_q4(x.cuda(), w), y.to(_st()))
+
+
 @pytest.mark.parametrize("symmetric", [True, False])
 @pytest.mark.parametrize("N,K,group", [(3, 32, 32), (37, 320, 64), (64, 1024, 128), (5, 4096, 128)])
 def test_quantize_and_dequantize_q4(N, K, group, symmetric):
