@@ -171,6 +171,13 @@ def test_rope_kv8_and_read(fmt, B, L, H, Hkv, D, layout):
     assert torch.equal(k.cpu(), (want[0].float() * want[1][..., None]).to(_st()))
 
 
+# rows of more heads than a workgroup of the writer takes
+@pytest.mark.parametrize("fmt", list(FMTS))
+@pytest.mark.parametrize("B,L,H,Hkv,D,layout", [(2, 5, 32, 32, 128, "bhsd"), (1, 3, 40, 8, 128, "bshd"), (2, 4, 64, 4, 64, "bhsd")])
+def test_rope_kv8_and_read_of_many_heads(fmt, B, L, H, Hkv, D, layout):
+    test_rope_kv8_and_read(fmt, B, L, H, Hkv, D, layout)
+
+
 @pytest.mark.parametrize("fmt", list(FMTS))
 def test_special_vectors(fmt):
     """Zero, tiny, huge and non-finite vectors; an infinity or NaN stays in its own vector."""
@@ -591,6 +598,12 @@ def test_logits_process(M, V, Lp, Lo, nb):
     xs[:, :V] = x.cuda()
     want = ops.logits_process(x.cuda(), **full)
     assert torch.equal(ops.logits_process(xs[:, :V], out=xs[:, :V], **full), want) and (xs[:, V] == 3.0).all()
+
+
+# so many rows that a workgroup takes 4096 tokens (rows of 16 bytes or not, slices that end early), and histories and biases of more than one round of loads
+@pytest.mark.parametrize("M,V,Lp,Lo,nb", [(260, 300, 20, 9, 3), (130, 8193, 12, 30, 2), (128, 4100, 15, 8, 0), (2, 900, 9001, 5003, 1024)])
+def test_logits_process_of_many_rows_and_long_histories(M, V, Lp, Lo, nb):
+    test_logits_process(M, V, Lp, Lo, nb)
 
 
 def test_logits_process_special_values():
