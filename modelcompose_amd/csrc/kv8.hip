@@ -243,14 +243,15 @@ __device__ __forceinline__ void attn8_append(const AttnParams8& p, int b, int hk
 // S^T = K Q^T: the keys are the rows (A operand, codes widened to 16 bits, exact), the heads the columns.  Of the 16 columns, column c and column c + 8 are
 // the same head; with row r of half t standing for key 8 (r >> 2) + 4 t + (r & 3), lane (c, g) ends up with the scores of keys 8 g .. 8 g + 7 of head
 // c & 7 - exactly the layout in which the next product O^T = V^T P^T wants its B operand, so the probabilities never leave the lane.  They
-// enter that product as bfloat16, a high part in columns 0 .. 7 and the remainder in columns 8 .. 15 (w = p * v_scale = hi + lo to 2^-17): the second half of
-// the columns carries the accuracy that 8 significant bits lack, at no instruction.  (bfloat16 also in the half-precision build: w has a wide range.)
+// enter that product as bfloat16, whose 8 significant bits are three parts of the fp32 weight w = p * v_scale = hi + mid + low, exactly: hi in columns 0 .. 7 and mid in columns
+// 8 .. 15 of one operand, low in columns 0 .. 7 of a second (bfloat16 also in the half-precision build: w has a wide range).  Two
+// parts (an error of 2^-17, nine times that of fp32 arithmetic in the sum) took 144.0 us where three take 145.5 (48 x 2809 keys), 12.4 against 12.6 (1 x 2809).
 // V^T's operand needs 8 keys of one element per lane: the bytes of two keys' rows are paired by v_perm.
 //
 // A workgroup of 4 waves takes chunks (attn8_chunk keys) blockIdx.y, + gridDim.y, ..; wave w the 32-key tiles w, w + 4, .. of a chunk, from a fresh (m, l, acc); the
 // waves are joined through LDS in wave order, the chunks by attn8_join in chunk order.  Which workgroup takes which chunk changes no bit.
 //
-// HBM-bound with many sequences: 48 x 2809 keys, 32 heads, D = 128 144 us = 5.8 TB/s (a kernel on the vector units, one head per workgroup: 157; the same loads
+// HBM-bound with many sequences: 48 x 2809 keys, 32 heads, D = 128 146 us = 5.7 TB/s (a kernel on the vector units, one head per workgroup: 157; the same loads
 // without the arithmetic: 138); 8 x 32768 keys, 32 heads over 8 92 us = 4.3 TB/s (757).  Latency-bound with few: 1 x 2809 keys 13 us, 3.8 of them the join.
 // Three waves per SIMD at D = 128 (168 registers): with two 162 us, with four the tile spills (229).
 template <int D, int FMT, bool KM>
@@ -411,19 +412,32 @@ __global__ __launch_bounds__(256, D == 128 ? 3 : 4) void attn_decode8_kernel(Att
         }
         const float base = m == -INFINITY ? 0.f : m;
         if constexpr (RAW) settle_v();
-        kv8_b16x8 pf;
+        u32x4 pf, pl;
+        const uint32_t upper = c < 8 ? 0u : 0xffffffffu;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            const float e = __builtin_amdgcn_exp2f(sc[j] - base);
-            l += e;
-            float w = e * vs[j];
-            if (MASKED && !((ok >> j) & 1u)) {                      // nothing of a masked key: not its scale, not its codes (either may be no number)
-                w = 0.f;
+        for (int j2 = 0; j2 < 4; ++j2) {
+            float w[2], rest[2], low[2];
 #pragma unroll
-                for (int u = 0; u < NU; ++u) vr[j][u] = 0u;
+            for (int i = 0; i < 2; ++i) {
+                const int j = 2 * j2 + i;
+                const float e = __builtin_amdgcn_exp2f(sc[j] - base);
+                l += e;
+                w[i] = e * vs[j];
+                if (MASKED && !((ok >> j) & 1u)) {                  // nothing of a masked key: not its scale, not its codes (either may be no number)
+                    w[i] = 0.f;
+#pragma unroll
+                    for (int u = 0; u < NU; ++u) vr[j][u] = 0u;
+                }
             }
-            const __bf16 hi = (__bf16)w;
-            pf[j] = c < 8 ? hi : (__bf16)(w - (float)hi);
+            const kv8_b16x2 hi = {(__bf16)w[0], (__bf16)w[1]};
+#pragma unroll
+            for (int i = 0; i < 2; ++i) rest[i] = w[i] - (float)hi[i];
+            const kv8_b16x2 mid = {(__bf16)rest[0], (__bf16)rest[1]};
+#pragma unroll
+            for (int i = 0; i < 2; ++i) low[i] = rest[i] - (float)mid[i];
+            const uint32_t h2 = __builtin_bit_cast(uint32_t, hi), m2 = __builtin_bit_cast(uint32_t, mid), l2 = __builtin_bit_cast(uint32_t, (kv8_b16x2){(__bf16)low[0], (__bf16)low[1]});
+            pf[j2] = (m2 & upper) | (h2 & ~upper);
+            pl[j2] = l2 & ~upper;
         }
         // V^T operands: row c of product i is element vd + i, of keys 8 g .. 8 g + 7
 #pragma unroll
@@ -440,7 +454,8 @@ __global__ __launch_bounds__(256, D == 128 ? 3 : 4) void attn_decode8_kernel(Att
                 u32x4 o;
 #pragma unroll
                 for (int k2 = 0; k2 < 4; ++k2) o[k2] = i & 1 ? kv8_pair<FMT, false, true>(pr[k2][i >> 1]) : kv8_pair<FMT, false, false>(pr[k2][i >> 1]);
-                acc[4 * u + i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(kv8_b16x8, o), pf, acc[4 * u + i], 0, 0, 0);
+                acc[4 * u + i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(kv8_b16x8, o), __builtin_bit_cast(kv8_b16x8, pl), acc[4 * u + i], 0, 0, 0);
+                acc[4 * u + i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(kv8_b16x8, o), __builtin_bit_cast(kv8_b16x8, pf), acc[4 * u + i], 0, 0, 0);
             }
         }
     };

@@ -751,3 +751,30 @@ def test_a_later_chunk_attends_to_what_is_read_back():
             assert ((out.cpu().double().view(B, n1, H, D)[b, :, h] - ref).abs() <= bound + 1e-6).all()
     last = ops.attn_decode8(q.view(B, n1, H, D)[:, -1], cache)                                # the last query as a decode step: the codes themselves
     near(last.view(B, H, D), *attend(qd[:, -1], [t.cpu() for t in (cache.k, cache.k_scale, cache.v, cache.v_scale)], [S] * B, 1 / math.sqrt(D)))
+
+
+def rounded(got, ref, err):
+    """Every element of got is ref rounded to the storage dtype, or - where ref lies within err of a border between two numbers - either of them."""
+    lo, hi = ((ref + s * err).to(_st()) for s in (-1, 1))
+    got = got.cpu()
+    bad = ~((got >= lo) & (got <= hi))
+    assert not bad.any(), f"{int(bad.sum())} of {bad.numel()} elements are not the rounded value"
+
+
+@pytest.mark.parametrize("fmt", list(FMTS))
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("n", [1, 7, 40])
+def test_weights_times_scales_keep_fp32(fmt, D, n):
+    """All scores equal (the queries are zero): the weights are 1, and what multiplies the codes is the values' scales alone.  Their 24 bits have to arrive:
+    two bfloat16 parts of them (2^-17) move a few in a thousand outputs over a border of the storage dtype, three parts are the scale itself."""
+    from modelcompose_amd import ops
+    g = _gen(200 + n + D)
+    B, H, Hkv = 24, 16, 8
+    cache, host = make_cache(g, B, Hkv, n, D, fmt)
+    host[3].mul_(1.0 + torch.rand(host[3].shape, generator=g))
+    cache.v_scale.copy_(host[3])
+    got = ops.attn_decode8(torch.zeros(B, H, D, dtype=_st(), device="cuda"), cache).view(B, Hkv, H // Hkv, D)
+    v = value(host[2], host[3])
+    ref, mag = v.mean(2), v.abs().mean(2)
+    # three exact products a key are added in fp32, then the two halves of the columns, 4 waves' partials, one division
+    rounded(got, ref[:, :, None].expand_as(got).contiguous(), ((3 * n + 12) * U * mag)[:, :, None])
