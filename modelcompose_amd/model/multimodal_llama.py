@@ -1255,13 +1255,14 @@ class MultimodalLlamaForCausalLM:
                         step_logits.append(lg)
             elif penalties is not None:
                 for s_ in range(max_new_tokens - 1 if not halted else 0):
+                    # the end of every row: before each token if hooks would see what follows it, else (a host sync) once in 16
+                    if not ignore_eos and (per_token or (s_ > 0 and s_ % 16 == 0)) and bool(((out[:, :1 + s_] == eos).any(dim=1)).all()):
+                        break
                     # (the step's own choice - an arg-max of the raw logits - is replaced; with a column of out to write it to)
                     lg = choose(self._decode(st, 1, out[:, 1:], s_, want_logits=True)[0], s_)
                     if return_step_logits:
                         step_logits.append(lg[None])
                     if per_token and hooks(2 + s_):
-                        break
-                    if not ignore_eos and s_ % 16 == 15 and bool(((out[:, :2 + s_] == eos).any(dim=1)).all()):      # host sync once in 16 tokens
                         break
             elif max_new_tokens > 1 and not halted:
                 if ignore_eos and not per_token:

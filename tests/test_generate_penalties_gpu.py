@@ -113,3 +113,40 @@ def test_refusals(case):
         model.generate(ids, modal_inputs=modal, max_new_tokens=2, num_beams=2, repetition_penalty=1.2)
     with pytest.raises(ValueError):
         model.generate(ids, modal_inputs=modal, max_new_tokens=2, ignore_eos=True, forced_ids=torch.zeros(len(ids), 2, dtype=torch.int64), presence_penalty=1.0)
+
+
+class _Recorder:
+    def __init__(self):
+        self.got, self.ended = [], False
+
+    def put(self, t):
+        self.got.append(t)
+
+    def end(self):
+        self.ended = True
+
+
+@pytest.mark.parametrize("kw", [dict(presence_penalty=1e4), dict(presence_penalty=1e4, do_sample=True, temperature=1.3, seed=3), dict(repetition_penalty=1.1, presence_penalty=1e4)])
+@pytest.mark.parametrize("last", [0, 1, 4, 17])
+def test_nothing_is_streamed_after_the_end(case, kw, last, monkeypatch):
+    """A streamer and the criteria see the answer and nothing behind it.  The presence penalty makes the tokens of a row distinct, so that any of them can be
+    declared the end of the sequence."""
+    model, ids, modal = case
+    one, pix = ids[:1], {"vision": modal["vision"][:1]}
+    free = model.generate(one, modal_inputs=pix, max_new_tokens=30, ignore_eos=True, **kw)[:, one.shape[1]:]
+    assert free[0].unique().numel() == 30
+    monkeypatch.setattr(model.config, "eos_token_id", int(free[0, last]))
+    rec, lengths = _Recorder(), []
+    res = model.generate(one, modal_inputs=pix, max_new_tokens=30, streamer=rec, stopping_criteria=[lambda s, _: bool(lengths.append(s.shape[1]))], **kw)
+    assert torch.equal(res[:, one.shape[1]:], free[:, :last + 1])
+    assert rec.ended and torch.equal(torch.stack(rec.got[1:], 1), free[:, :last + 1].cpu())
+    assert lengths == [one.shape[1] + i + 1 for i in range(last + 1)]
+    assert torch.equal(res, model.generate(one, modal_inputs=pix, max_new_tokens=30, **kw))            # and the loop without hooks
+
+
+def test_streaming_goes_on_until_every_row_has_ended(case):
+    model, ids, modal = case
+    eos = model.config.eos_token_id
+    rec = _Recorder()
+    res = model.generate(ids, modal_inputs=modal, max_new_tokens=20, streamer=rec, logit_bias={eos: 1e4})
+    assert res.shape[1] == ids.shape[1] + 1 and len(rec.got) == 2 and (rec.got[1] == eos).all()
