@@ -1136,7 +1136,7 @@ class MultimodalLlamaForCausalLM:
         do_sample=True applies transformers 4.31's warpers in their order (temperature, top_k - GenerationConfig default 50, pass
         top_k=0 to disable - then top_p) and draws with a Philox stream keyed by `seed` (kwarg; default: drawn from torch's global
         generator, so torch.manual_seed makes runs repeatable).  num_beams > 1: beam search (_beam_search; kwargs length_penalty, early_stopping).
-        repetition_penalty (over the text prompt and the generated ids: RepetitionPenaltyLogitsProcessor), presence_penalty, frequency_penalty
+        repetition_penalty (over the text prompt, without padding, and the generated ids: RepetitionPenaltyLogitsProcessor), presence_penalty, frequency_penalty
         (generated ids) and logit_bias ({token id: bias}) change the logits before either rule (ops.logits_process), one launch sequence per token;
         return_step_logits then returns the processed ones."""
         penalties = _logits_options(kw, self.config.vocab_size)
@@ -1206,7 +1206,10 @@ class MultimodalLlamaForCausalLM:
                 out.zero_()
             if penalties is not None:
                 pen = penalties.tensors(B, self.device)
-                prompt = input_ids.to(self.device, torch.int64).contiguous()
+                prompt = input_ids.to(self.device, torch.int64)
+                if attention_mask is not None:                       # padding is no part of the prompt (ids outside the vocabulary count for nothing)
+                    prompt = prompt.masked_fill(~attention_mask.to(self.device, torch.bool), -1)
+                prompt = prompt.contiguous()
 
                 def choose(logits, s_):                              # token s_ + 1 from the logits after s_ + 1 generated tokens (s_ = -1: the first)
                     lg = ops.logits_process(logits, prompt_ids=prompt, output_ids=out[:, :s_ + 1] if s_ >= 0 else None, **pen)

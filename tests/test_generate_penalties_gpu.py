@@ -150,3 +150,29 @@ def test_streaming_goes_on_until_every_row_has_ended(case):
     rec = _Recorder()
     res = model.generate(ids, modal_inputs=modal, max_new_tokens=20, streamer=rec, logit_bias={eos: 1e4})
     assert res.shape[1] == ids.shape[1] + 1 and len(rec.got) == 2 and (rec.got[1] == eos).all()
+
+
+@pytest.mark.parametrize("left", [False, True])
+@pytest.mark.parametrize("kw", [dict(repetition_penalty=1.8), dict(repetition_penalty=0.5, frequency_penalty=0.3)])
+def test_padding_is_no_part_of_the_prompt(case, left, kw):
+    """What a row is padded with is not penalised: the scores are the raw logits of the same padded batch with the penalties of the tokens that the mask leaves.  Padded behind
+    its end, a row has the tokens and scores it has alone.  (Padded before its start it need not: with modal tokens the spliced mask is the text's, extended on the left.)"""
+    model, ids, modal = case
+    n, L = 8, ids.shape[1]
+    run = lambda i, m, **more: model.generate(i, modal_inputs=m, max_new_tokens=n, ignore_eos=True, return_step_logits=True, **kw, **more)
+    alone = [run(ids[b:b + 1], {"vision": modal["vision"][b:b + 1]}) for b in range(len(ids))]
+    for pad in (0, int(alone[0][0][0, L]), model.config.eos_token_id):
+        wide = torch.full((len(ids), L + 3), pad, dtype=ids.dtype, device=ids.device)
+        mask = torch.zeros(wide.shape, dtype=torch.bool, device=ids.device)
+        at = slice(3, L + 3) if left else slice(0, L)
+        wide[:, at], mask[:, at] = ids, True
+        res, lg = run(wide, modal, attention_mask=mask)
+        new = res[:, L + 3:]
+        _, raw = model.generate(wide, modal_inputs=modal, attention_mask=mask, max_new_tokens=n, ignore_eos=True, forced_ids=new, return_step_logits=True)
+        want = _processed(raw.cpu(), ids.cpu(), new.cpu(), kw["repetition_penalty"], 0.0, kw.get("frequency_penalty", 0.0), {})
+        # four fp32 roundings at most, as in test_chosen_tokens_and_scores
+        mag = raw.cpu().double().abs() * 2 + want.abs() + 3 * n * kw.get("frequency_penalty", 0.0)
+        assert ((lg.cpu().double() - want).abs() <= 4 * 2.0 ** -24 * mag).all(), pad
+        if not left:
+            for b, (r, l) in enumerate(alone):
+                assert torch.equal(new[b], r[0, L:]) and torch.equal(lg[b], l[0])
