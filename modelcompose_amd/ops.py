@@ -5,6 +5,7 @@ from __future__ import annotations
 import contextlib
 import ctypes as C
 import math
+import operator
 import threading
 from typing import Optional, Sequence
 
@@ -666,11 +667,22 @@ def _arg(t, name, index, dtype, shape):
     return t.data_ptr()
 
 
+def _fixed(*names):
+    """Class decorator: the public fields are read-only views of the private slots.  The C structs hold the addresses, strides and sizes of construction, so a
+    field that could be replaced would be ignored by the next call, and the memory it held would be freed under it."""
+    def wrap(cls):
+        for n in names:
+            setattr(cls, n, property(operator.attrgetter("_" + n)))
+        return cls
+    return wrap
+
+
+@_fixed("codes", "scales", "zeros", "N", "K", "group", "index")
 class Q4Weight:
     """A linear weight in 4 bits: W[n, k] = scales[n, k // group] * (code[n, k] - zeros[n, k // group]).
     codes uint8 [N, K / 2] (two codes to a byte, even k in the low half), scales [N, K / group] in the storage dtype, zeros uint8 [N, K / group] or None (8);
-    group = K // scales.shape[1]: 32, 64 or 128.  bias (storage dtype [N]) as in PackedWeight."""
-    __slots__ = ("codes", "scales", "zeros", "bias", "N", "K", "group", "index", "_c")
+    group = K // scales.shape[1]: 32, 64 or 128.  bias (storage dtype [N]) as in PackedWeight; it may be set, the other fields are those of construction."""
+    __slots__ = ("_codes", "_scales", "_zeros", "_bias", "_N", "_K", "_group", "_index", "_c")
 
     def __init__(self, codes, scales, zeros=None, bias=None):
         index = _device(codes, "codes")
@@ -685,17 +697,26 @@ class Q4Weight:
         pc = _arg(codes, "codes", index, _U8, (N, half))
         ps = _arg(scales, "scales", index, BF16, (N, G))
         pz = 0 if zeros is None else _arg(zeros, "zeros", index, _U8, (N, G))
-        if bias is not None:
-            _arg(bias, "bias", index, BF16, (N,))
         # (a single row has no row stride: torch may report anything there)
         one = N < 2
-        self.codes, self.scales, self.zeros, self.bias, self.N, self.K, self.group, self.index = codes, scales, zeros, bias, N, K, group, index
+        self._codes, self._scales, self._zeros, self._N, self._K, self._group, self._index = codes, scales, zeros, N, K, group, index
+        self.bias = bias
         self._c = _lib.Q4WeightC(pc, half if one else codes.stride(0), ps, G if one else scales.stride(0), pz,
                                  0 if zeros is None else G if one else zeros.stride(0), N, K, group)
 
     @property
+    def bias(self):
+        return self._bias
+
+    @bias.setter
+    def bias(self, bias):
+        if bias is not None:
+            _arg(bias, "bias", self._index, BF16, (self._N,))
+        self._bias = bias
+
+    @property
     def nbytes(self):
-        return sum(t.numel() * t.element_size() for t in (self.codes, self.scales, self.zeros) if t is not None)
+        return sum(t.numel() * t.element_size() for t in (self._codes, self._scales, self._zeros) if t is not None)
 
 
 def quantize_q4(w: torch.Tensor, group: int = 128, symmetric: bool = True, bias: Optional[torch.Tensor] = None) -> Q4Weight:
@@ -716,9 +737,9 @@ def quantize_q4(w: torch.Tensor, group: int = 128, symmetric: bool = True, bias:
 
 def dequantize_q4(w: Q4Weight) -> PackedWeight:
     """The 16-bit PackedWeight of a 4-bit weight (each element rounded once): linear() with more than 64 rows."""
-    out = torch.empty(packed_elems(w.N, w.K), dtype=BF16, device=w.codes.device)
-    _call("mc_dequantize_q4_bf16", w.index, C.byref(w._c), out.data_ptr())
-    return PackedWeight(out, w.N, w.K, w.bias)
+    out = torch.empty(packed_elems(w._N, w._K), dtype=BF16, device=w._codes.device)
+    _call("mc_dequantize_q4_bf16", w._index, C.byref(w._c), out.data_ptr())
+    return PackedWeight(out, w._N, w._K, w._bias)
 
 
 def linear_q4(x: torch.Tensor, w: Q4Weight, residual: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None, out_f32: bool = False,
@@ -729,12 +750,12 @@ def linear_q4(x: torch.Tensor, w: Q4Weight, residual: Optional[torch.Tensor] = N
     index = _device(x, "x")
     if x.dim() != 2:
         raise ValueError("x must be 2-D [M, K]")
-    M, N, dt = x.shape[0], w.N, _F32 if out_f32 else BF16
-    px = _arg(x, "x", index, BF16, (M, w.K))
+    M, N, dt = x.shape[0], w._N, _F32 if out_f32 else BF16
+    px = _arg(x, "x", index, BF16, (M, w._K))
     if M > 64:
         raise ValueError(f"linear_q4 takes at most 64 rows, got {M}: use linear(x, dequantize_q4(w))")
-    if w.index != index:
-        raise ValueError(f"the weight is on device {w.index}, x on device {index}")
+    if w._index != index:
+        raise ValueError(f"the weight is on device {w._index}, x on device {index}")
     if out is None:
         out = torch.empty((M, N), dtype=_F32, device=x.device) if out_f32 else x.new_empty((M, N))
         po, ldo = out.data_ptr(), N
@@ -743,16 +764,18 @@ def linear_q4(x: torch.Tensor, w: Q4Weight, residual: Optional[torch.Tensor] = N
     pr, ldr = (0, 0) if residual is None else (_arg(residual, "residual", index, BF16, (M, N)), residual.stride(0))
     if M:
         # (mc_linear_q4_workspace_bytes)
-        ws = torch.empty((M + 15) // 16 * 16 * w.K, dtype=BF16, device=x.device) if M > 16 else None
-        _call("mc_linear_q4_bf16", index, px, x.stride(0) if M > 1 else w.K, w._c, w.bias.data_ptr() if bias and w.bias is not None else 0, pr, ldr, po, ldo, M,
+        ws = torch.empty((M + 15) // 16 * 16 * w._K, dtype=BF16, device=x.device) if M > 16 else None
+        _call("mc_linear_q4_bf16", index, px, x.stride(0) if M > 1 else w._K, w._c, w._bias.data_ptr() if bias and w._bias is not None else 0, pr, ldr, po, ldo, M,
               1 if out_f32 else 0, 0 if ws is None else ws.data_ptr())
     return out
 
 
+@_fixed("k", "k_scale", "v", "v_scale", "B", "Hkv", "S", "D", "index")
 class Kv8Cache:
     """An 8-bit KV cache of one layer: codes k, v [B, Hkv, S, D] (torch.float8_e4m3fn or torch.int8, equal strides, head_dim contiguous) and their fp32
-    scales k_scale, v_scale [B, Hkv, S], one per vector.  kv8_cache() makes one; slices over the batch of an existing one are caches too."""
-    __slots__ = ("k", "k_scale", "v", "v_scale", "B", "Hkv", "S", "D", "index", "_c")
+    scales k_scale, v_scale [B, Hkv, S], one per vector.  kv8_cache() makes one; slices over the batch of an existing one are caches too.
+    The fields are those of construction: a grown cache is a new one."""
+    __slots__ = ("_k", "_k_scale", "_v", "_v_scale", "_B", "_Hkv", "_S", "_D", "_index", "_c")
     _formats = {torch.float8_e4m3fn: 1, torch.int8: 2}
 
     def __init__(self, k, k_scale, v, v_scale):
@@ -771,12 +794,12 @@ class Kv8Cache:
         zb, zh = ss[0] if B > 1 else 1, ss[1] if Hkv > 1 else 1
         if not (sb > 0 and sh > 0 and sp > 0 and zb > 0 and zh > 0):
             raise ValueError("a cache has no broadcast dimensions")
-        self.k, self.k_scale, self.v, self.v_scale, self.B, self.Hkv, self.S, self.D, self.index = k, k_scale, v, v_scale, B, Hkv, S, D, index
+        self._k, self._k_scale, self._v, self._v_scale, self._B, self._Hkv, self._S, self._D, self._index = k, k_scale, v, v_scale, B, Hkv, S, D, index
         self._c = _lib.Kv8CacheC(pk, pks, pv, pvs, sb, sh, sp, zb, zh, B, Hkv, S, D, fmt)
 
     @property
     def nbytes(self):
-        return sum(t.numel() * t.element_size() for t in (self.k, self.k_scale, self.v, self.v_scale))
+        return sum(t.numel() * t.element_size() for t in (self._k, self._k_scale, self._v, self._v_scale))
 
 
 def kv8_cache(B, Hkv, S, D, device="cuda", dtype=torch.float8_e4m3fn) -> Kv8Cache:
@@ -787,12 +810,12 @@ def kv8_cache(B, Hkv, S, D, device="cuda", dtype=torch.float8_e4m3fn) -> Kv8Cach
 
 
 def _rope_args(qkv, cos, sin, cache, H, rows):
-    index, width = _device(qkv, "qkv"), (H + 2 * cache.Hkv) * cache.D
+    index, width = _device(qkv, "qkv"), (H + 2 * cache._Hkv) * cache._D
     p = _arg(qkv, "qkv", index, BF16, (rows, width))
-    if cache.index != index:
-        raise ValueError(f"the cache is on device {cache.index}, qkv on device {index}")
+    if cache._index != index:
+        raise ValueError(f"the cache is on device {cache._index}, qkv on device {index}")
     n_pos = cos.shape[0]
-    pc, ps = _arg(cos, "cos", index, _F32, (n_pos, cache.D // 2)), _arg(sin, "sin", index, _F32, (n_pos, cache.D // 2))
+    pc, ps = _arg(cos, "cos", index, _F32, (n_pos, cache._D // 2)), _arg(sin, "sin", index, _F32, (n_pos, cache._D // 2))
     if not (cos.is_contiguous() and sin.is_contiguous()):
         raise ValueError("cos and sin must be contiguous")
     return index, p, qkv.stride(0) if rows > 1 else width, pc, ps, n_pos
@@ -806,8 +829,8 @@ def rope_kv8(qkv, row_b, row_pos, row_t, cos, sin, q_out, cache: Kv8Cache, H, Lq
     index, p, ld, pc, ps, n_pos = _rope_args(qkv, cos, sin, cache, H, M)
     rb, rp, rt = _arg(row_b, "row_b", index, _I32, (M,)), _arg(row_pos, "row_pos", index, _I32, (M,)), _arg(row_t, "row_t", index, _I32, (M,))
     pq = _arg(q_out, "q_out", index, BF16, q_out.shape)
-    if not q_out.is_contiguous() or q_out.numel() != cache.B * Lq * H * cache.D:
-        raise ValueError(f"q_out must hold {cache.B} x {Lq} contiguous rows of {H * cache.D}")
+    if not q_out.is_contiguous() or q_out.numel() != cache._B * Lq * H * cache._D:
+        raise ValueError(f"q_out must hold {cache._B} x {Lq} contiguous rows of {H * cache._D}")
     if M:
         _call("mc_rope_kv8", index, p, ld, rb, rp, rt, pc, ps, n_pos, pq, cache._c, M, H, Lq)
     return q_out
@@ -816,14 +839,14 @@ def rope_kv8(qkv, row_b, row_pos, row_t, cos, sin, q_out, cache: Kv8Cache, H, Lq
 def kv8_read(cache: Kv8Cache, n=None, kv_lens=None):
     """The first n (default: all) positions in the storage dtype: (k, v) [B, Hkv, n, D]; positions from kv_lens[b] on are zeros.  What attn_prefill reads when a
     later chunk of a prompt attends to keys that are in the cache already."""
-    n = cache.S if n is None else int(n)
-    pl = 0 if kv_lens is None else _arg(kv_lens, "kv_lens", cache.index, _I32, (cache.B,))
-    if n < 0 or n > cache.S:
-        raise ValueError(f"{n} positions of a cache of {cache.S}")
-    k = torch.empty((cache.B, cache.Hkv, n, cache.D), dtype=BF16, device=cache.k.device)
+    n = cache._S if n is None else int(n)
+    pl = 0 if kv_lens is None else _arg(kv_lens, "kv_lens", cache._index, _I32, (cache._B,))
+    if n < 0 or n > cache._S:
+        raise ValueError(f"{n} positions of a cache of {cache._S}")
+    k = torch.empty((cache._B, cache._Hkv, n, cache._D), dtype=BF16, device=cache._k.device)
     v = torch.empty_like(k)
     if n:
-        _call("mc_kv8_read", cache.index, cache._c, pl, n, k.data_ptr(), v.data_ptr())
+        _call("mc_kv8_read", cache._index, cache._c, pl, n, k.data_ptr(), v.data_ptr())
     return k, v
 
 
@@ -842,7 +865,7 @@ def _decode8_scratch(B, H, D, S):
 def _decode8(name, head, x, cache, H, kv_lens, out, scale, key_valid):
     """The arguments that attn_decode8 and attn_decode8_rope share, and the call.  The scratch is the caching allocator's: calls in flight on other streams, and
     captured graphs, have their own."""
-    B, D, S, index = cache.B, cache.D, cache.S, cache.index
+    B, D, S, index = cache._B, cache._D, cache._S, cache._index
     pl = 0 if kv_lens is None else _arg(kv_lens, "kv_lens", index, _I32, (B,))
     pm = ms = 0
     if key_valid is not None:
@@ -868,10 +891,10 @@ def attn_decode8(q, cache: Kv8Cache, kv_lens=None, out=None, scale=None, key_val
     if q.dim() != 3:
         raise ValueError("q must be [B, H, D]")
     H = q.shape[1]
-    pq = _arg(q, "q", index, BF16, (cache.B, H, cache.D))
-    if cache.index != index:
-        raise ValueError(f"the cache is on device {cache.index}, q on device {index}")
-    return _decode8("mc_attn_decode8", (pq, q.stride(0) if cache.B > 1 else cache.D, q.stride(1) if H > 1 else cache.D), q, cache, H, kv_lens, out, scale, key_valid)
+    pq = _arg(q, "q", index, BF16, (cache._B, H, cache._D))
+    if cache._index != index:
+        raise ValueError(f"the cache is on device {cache._index}, q on device {index}")
+    return _decode8("mc_attn_decode8", (pq, q.stride(0) if cache._B > 1 else cache._D, q.stride(1) if H > 1 else cache._D), q, cache, H, kv_lens, out, scale, key_valid)
 
 
 def attn_decode8_rope(qkv, cos, sin, cache: Kv8Cache, kv_lens, H, out=None, scale=None, key_valid=None):
@@ -879,7 +902,7 @@ def attn_decode8_rope(qkv, cos, sin, cache: Kv8Cache, kv_lens, H, out=None, scal
     are rotated, appended to the cache and attended.  A sequence with kv_lens[b] outside 1 .. min(S, rows of cos) is left alone: zeros, nothing written."""
     if kv_lens is None:
         raise ValueError("kv_lens is needed: it places the new token")
-    index, p, ld, pc, ps, n_pos = _rope_args(qkv, cos, sin, cache, H, cache.B)
+    index, p, ld, pc, ps, n_pos = _rope_args(qkv, cos, sin, cache, H, cache._B)
     return _decode8("mc_attn_decode8_rope", (p, ld, pc, ps, n_pos), qkv, cache, H, kv_lens, out, scale, key_valid)
 
 

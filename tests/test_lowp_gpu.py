@@ -778,3 +778,33 @@ def test_weights_times_scales_keep_fp32(fmt, D, n):
     ref, mag = v.mean(2), v.abs().mean(2)
     # three exact products a key are added in fp32, then the two halves of the columns, 4 waves' partials, one division
     rounded(got, ref[:, :, None].expand_as(got).contiguous(), ((3 * n + 12) * U * mag)[:, :, None])
+
+
+def test_the_fields_of_a_weight_and_a_cache_cannot_be_replaced():
+    """The kernels get the addresses, strides and sizes of construction: another tensor in a field's place would be ignored, and the old one's memory freed."""
+    from modelcompose_amd import ops
+    g = _gen(51)
+    cache = ops.kv8_cache(2, 2, 16, 64)
+    codes, scales, z = random_q4(g, 40, 64, 32, True)
+    w = ops.Q4Weight(codes.cuda(), scales.cuda(), z.cuda())
+    for o, names in ((cache, ("k", "k_scale", "v", "v_scale", "B", "Hkv", "S", "D", "index")), (w, ("codes", "scales", "zeros", "N", "K", "group", "index"))):
+        for n in names:
+            old = getattr(o, n)
+            with pytest.raises(AttributeError):
+                setattr(o, n, old)
+            with pytest.raises(AttributeError):
+                delattr(o, n)
+            assert getattr(o, n) is old or getattr(o, n) == old
+    with pytest.raises(AttributeError):
+        cache.other = 1
+    # the bias is read at each call: it may be set, if it is one
+    x, bias = _rand(g, 3, 64).cuda(), _rand(g, 40).cuda()
+    plain = ops.linear_q4(x, w, out_f32=True)
+    w.bias = bias
+    assert torch.equal(ops.linear_q4(x, w, out_f32=True), plain + bias.float())
+    for bad in (bias[:39], bias.float(), bias.cpu(), torch.zeros(80, dtype=_st(), device="cuda")[::2]):
+        with pytest.raises(ValueError):
+            w.bias = bad
+        assert w.bias is bias
+    w.bias = None
+    assert torch.equal(ops.linear_q4(x, w, out_f32=True), plain)
