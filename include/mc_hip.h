@@ -417,7 +417,8 @@ typedef struct mc_q4_weight {
     int N, K, group;
 } mc_q4_weight;
 /* out[M, N] = x[M, K] W^T (+ bias) (+ residual): at most 64 rows; out 16-bit, or fp32 with out_f32.  Codes are multiplied as exact integers and summed in
- * fp32 per group, the zero point is taken out as zero * sum(x), then scaled: an infinity in a row of x gives NaN.  A row's result does not depend on M.
+ * fp32 per group, the zero point is taken out as zero * sum(x), then scaled; an output for which these sums are infinite or NaN is computed from the
+ * definition (an infinity in x gives an infinity, or NaN where the weight is 0).  A row's result does not depend on M.
  * out may be residual, but may not overlap x. */
 int mc_linear_q4_bf16(const void* x, int64_t ldx, const mc_q4_weight* w, const void* bias, const void* residual, int64_t ldr, void* out, int64_t ldo,
                       int M, int out_f32, void* workspace, void* stream);

@@ -15,6 +15,26 @@ struct Q4Params {
     const bf16_t* xp;                        // x in operand order (pack_x_kernel), for more than 16 rows
 };
 
+// y[m][n] from the definition, in 64 bits: for an output whose sums over the bare codes came out infinite or NaN.  sum q x and z sum x both pass the range where
+// sum (q - z) x need not (an infinity in x has the sign of q - z, not inf - inf; 15 x overflows before s (q - z) x does).  Looking for such an output costs 0.1 us of
+// 1 x 4096 x 4096 (4.4 -> 4.5) and 0.15 of 48 x 12288 x 4096 (16.8 -> 16.95).
+__device__ float q4_define(const Q4Params& p, int m, int n) {
+    double y = 0;
+    const uint8_t* row = p.codes + n * p.ldc;
+    const bf16_t* x = p.x + m * p.ldx;
+#pragma unroll 1
+    for (int k = 0; k < p.K; k += 8) {
+        const int g = k >> p.gshift;
+        const uint32_t w = *(const uint32_t*)(row + k / 2);
+        const bf16x8 v = *(const bf16x8*)(x + k);
+        const double s = (double)(float)p.scales[n * p.lds + g];
+        const int z = p.zeros ? p.zeros[n * p.ldz + g] : 8;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) y = fma(s * (double)((int)((w >> (4 * j)) & 15u) - z), (double)(float)v[j], y);
+    }
+    return (float)y;
+}
+
 __device__ __forceinline__ void q4_store(const Q4Params& p, int m, int n, float y) {
     if (p.bias) y += (float)p.bias[n];
     if (p.residual) y += (float)p.residual[m * p.ldr + n];
@@ -255,13 +275,20 @@ __global__ __launch_bounds__(W * 64) void linear_q4_kernel(Q4Params p) {
         f32x4 v = *(f32x4*)&red[0][q][lane][0];
 #pragma unroll
         for (int w = 1; w < H; ++w) v += *(f32x4*)&red[w][q][lane][0];
-        const int n = (blockIdx.x * R + r) * 16 + c;
-        if (n < p.N)
-#pragma unroll
+        const int n = (blockIdx.x * R + r) * 16 + c, m0 = b * 16 + 4 * g;
+        if (n >= p.N) continue;
+        if (!(fabsf(v[0]) < INFINITY && fabsf(v[1]) < INFINITY && fabsf(v[2]) < INFINITY && fabsf(v[3]) < INFINITY)) {
+#pragma unroll 1
             for (int t = 0; t < 4; ++t) {
-                const int m = b * 16 + 4 * g + t;
-                if (m < p.M) q4_store(p, m, n, v[t]);
+                float y = t == 0 ? v[0] : t == 1 ? v[1] : t == 2 ? v[2] : v[3];
+                if (fabsf(y) < INFINITY || m0 + t >= p.M) continue;
+                y = q4_define(p, m0 + t, n);
+                v[0] = t == 0 ? y : v[0]; v[1] = t == 1 ? y : v[1]; v[2] = t == 2 ? y : v[2]; v[3] = t == 3 ? y : v[3];
             }
+        }
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+            if (m0 + t < p.M) q4_store(p, m0 + t, n, v[t]);
     }
 }
 

@@ -745,8 +745,8 @@ def dequantize_q4(w: Q4Weight) -> PackedWeight:
 def linear_q4(x: torch.Tensor, w: Q4Weight, residual: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None, out_f32: bool = False,
               bias: bool = True) -> torch.Tensor:
     """out[M, N] = x W^T (+ bias) (+ residual) for at most 64 rows x [M, K] (the decode step's form of linear(); larger launches: linear(x,
-    dequantize_q4(w)), with x padded to its Kp).  fp32 sums; the codes enter as exact integers, the zero point as zero * sum(x) (an infinity in x gives NaN).
-    A row's bits do not depend on M.  out may be the residual, but may not overlap x."""
+    dequantize_q4(w)), with x padded to its Kp).  fp32 sums; the codes enter as exact integers, the zero point as zero * sum(x); an infinity in x gives the
+    infinities and NaN of linear().  A row's bits do not depend on M.  out may be the residual, but may not overlap x."""
     index = _device(x, "x")
     if x.dim() != 2:
         raise ValueError("x must be 2-D [M, K]")

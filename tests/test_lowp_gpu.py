@@ -808,3 +808,51 @@ def test_the_fields_of_a_weight_and_a_cache_cannot_be_replaced():
         assert w.bias is bias
     w.bias = None
     assert torch.equal(ops.linear_q4(x, w, out_f32=True), plain)
+
+
+@pytest.mark.parametrize("M", [1, 5, 16, 20, 50])
+@pytest.mark.parametrize("N,K,group,zeros", [(70, 224, 32, True), (33, 1024, 128, False), (4130, 320, 64, True), (8200, 256, 64, False)])
+def test_linear_q4_of_infinities_and_the_largest_numbers(M, N, K, group, zeros):
+    """An infinity in x gives what the definition gives: an infinity of the weight's sign, NaN where the weight is zero or two disagree; finite numbers whose products with
+    the bare codes pass the range of fp32 give the finite sum.  The other rows do not notice."""
+    from modelcompose_amd import ops
+    g = _gen(N + M)
+    codes, scales, z = random_q4(g, N, K, group, zeros)
+    x = _rand(g, M, K)
+    clean = x.clone()
+    hit = sorted({0, M // 2, M - 1})
+    top = torch.finfo(_st()).max
+    for i, m in enumerate(hit):
+        if i == 0:
+            x[m, K - 1] = math.inf
+        elif i == 1:
+            x[m, 3], x[m, K // 2] = -math.inf, math.inf
+        else:
+            x[m, 1::2] = top
+            x[m, 0::2] = -top
+    w = ops.Q4Weight(codes.cuda(), scales.cuda(), None if z is None else z.cuda())
+    y = ops.linear_q4(x.cuda(), w, out_f32=True).cpu()
+    q = torch.stack([codes & 15, codes >> 4], -1).view(N, -1).double()
+    wt = (q - (8.0 if z is None else z.double().repeat_interleave(group, 1))) * scales.double().repeat_interleave(group, 1)
+    for m in hit:
+        t = x[m].double() * wt                                         # (0 * inf is NaN, as in any product)
+        ref = t.sum(1)
+        assert torch.equal(torch.isnan(y[m]), torch.isnan(ref)) and torch.equal(torch.isposinf(y[m]), torch.isposinf(ref.float())) and torch.equal(torch.isneginf(y[m]), torch.isneginf(ref.float()))
+        fin = torch.isfinite(ref.float())
+        assert ((y[m].double() - ref).abs()[fin] <= ((K + 16) * U * (x[m].double().abs() @ (q + 15).mul(scales.double().repeat_interleave(group, 1)).t()))[fin]).all()
+    rest = [m for m in range(M) if m not in hit]
+    assert torch.equal(y[rest], ops.linear_q4(clean.cuda(), w, out_f32=True).cpu()[rest])
+    assert torch.equal(ops.linear_q4(x[M - 1:].cuda(), w, out_f32=True)[0].cpu().nan_to_num(nan=7.0), y[M - 1].nan_to_num(nan=7.0))
+
+
+def test_linear_q4_of_infinities_is_the_prompt_form():
+    """The 16-bit form of the same weight gives the same infinities and NaN."""
+    from modelcompose_amd import ops
+    g = _gen(61)
+    codes, scales, z = random_q4(g, 132, 256, 64, True)
+    w = ops.Q4Weight(codes.cuda(), scales.cuda(), z.cuda())
+    x = _rand(g, 9, 256)
+    x[2, 100], x[5, 0] = math.inf, -math.inf
+    a, b = ops.linear_q4(x.cuda(), w).float(), ops.linear(x.cuda(), ops.dequantize_q4(w)).float()
+    assert torch.equal(torch.isnan(a), torch.isnan(b)) and torch.equal(torch.isposinf(a), torch.isposinf(b)) and torch.equal(torch.isneginf(a), torch.isneginf(b))
+    assert torch.isinf(a[2]).any() and torch.isinf(a[5]).any()
