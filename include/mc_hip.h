@@ -398,7 +398,7 @@ int mc_log_softmax_f32(const float* logits, int64_t ld, float* out, int64_t ldo,
  *   l = seen ? (l > 0 ? l / repetition[m] : l * repetition[m]) : l;   l -= frequency[m] * c + presence[m] * (c > 0);
  *   l += sum of bias[m][i] over bias_ids[m][i] == t;   l = -inf unless bit t & 31 of allowed[m][t >> 5] is set.
  * Every array but logits / out may be NULL: that part is left out (repetition 1, the penalties 0, no bias, everything allowed).  Ids outside
- * [0, V) are ignored; lengths are clipped to [0, cols]; NULL lengths = cols.  All rows in row strides (elements). */
+ * [0, V) are ignored (so they pad ragged lists); lengths are clipped to [0, cols]; NULL lengths = cols.  All rows in row strides (elements). */
 typedef struct mc_logits_args {
     const float* logits; int64_t ld; float* out; int64_t ld_out; int M, V;
     const int64_t* prompt_ids; int64_t ld_prompt; const int32_t* prompt_lens; int prompt_cols;

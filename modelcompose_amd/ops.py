@@ -911,7 +911,8 @@ def logits_process(logits, prompt_ids=None, prompt_lens=None, output_ids=None, o
     """Penalties, biases and a token mask on logits [M, V] fp32, before argmax() / sample_step() (out=logits: in place).
     prompt_ids / output_ids int64 [M, n] with optional int32 lengths [M]: the repetition penalty (l / r or l * r) reads both, frequency * count + presence
     only the output ids.  The penalties are fp32 tensors [M]; bias_ids int32 [M, n] with bias fp32 [M, n] (a token may be listed twice: the biases add up);
-    allowed int32 [M, ceil(V / 32)]: bit t & 31 of word t >> 5 clear = -inf.  Ids outside [0, V) are ignored.
+    allowed int32 [M, ceil(V / 32)]: bit t & 31 of word t >> 5 clear = -inf.  Ids outside [0, V) are ignored:
+    ragged lists are padded with -1.
     out is logits itself or does not overlap it."""
     index = _device(logits, "logits")
     if logits.dim() != 2:

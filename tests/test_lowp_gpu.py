@@ -856,3 +856,59 @@ def test_linear_q4_of_infinities_is_the_prompt_form():
     a, b = ops.linear_q4(x.cuda(), w).float(), ops.linear(x.cuda(), ops.dequantize_q4(w)).float()
     assert torch.equal(torch.isnan(a), torch.isnan(b)) and torch.equal(torch.isposinf(a), torch.isposinf(b)) and torch.equal(torch.isneginf(a), torch.isneginf(b))
     assert torch.isinf(a[2]).any() and torch.isinf(a[5]).any()
+
+
+def _same_id_row(n, V, same):
+    g = _gen(n)
+    x = torch.randn(1, V, generator=g)
+    ids = torch.full((1, n), 5, dtype=torch.int32) if same else torch.randperm(V, generator=g)[:n].int()[None]
+    return x, ids, torch.randn(1, n, generator=g)
+
+
+@pytest.mark.parametrize("n", [1, 2, 3, 17, 64, 65, 100, 513, 1023, 1024])
+@pytest.mark.parametrize("V", [1024, 40000])
+def test_biases_of_one_token_add_up_in_the_order_of_the_list(n, V):
+    """Up to 1024 times the same token, alone or between others: fp32 additions in list order, bit for bit."""
+    from modelcompose_amd import ops
+    x, ids, bias = _same_id_row(n, V, True)
+    y = ops.logits_process(x.cuda(), bias_ids=ids.cuda(), bias=bias.cuda()).cpu()
+    total = torch.zeros(())
+    for v in bias[0]:
+        total = total + v
+    want = x.clone()
+    want[0, 5] += total
+    assert torch.equal(y, want)
+    g = _gen(n + 1)
+    M = 3
+    x = torch.randn(M, V, generator=g)
+    ids = torch.randint(-1, 12, (M, n), generator=g).int() * (V // 11)             # a few tokens many times, over all slices, some outside
+    bias = torch.randn(M, n, generator=g)
+    y = ops.logits_process(x.cuda(), bias_ids=ids.cuda(), bias=bias.cuda()).cpu()
+    want = x.clone()
+    for m in range(M):
+        total = {}
+        for t, v in zip(ids[m].tolist(), bias[m]):
+            total[t] = total.get(t, torch.zeros(())) + v
+        for t, v in total.items():
+            if 0 <= t < V:
+                want[m, t] += v
+    assert torch.equal(y, want)
+
+
+def test_repeated_biases_cost_about_what_different_ones_do():
+    """1024 entries of one token (a ragged list padded with one id) against 1024 tokens: a sum over the list, not a walk of the list per entry."""
+    from modelcompose_amd import ops
+    times = []
+    for same in (False, True):
+        x, ids, bias = (t.cuda() for t in _same_id_row(1024, 2048, same))
+        out = torch.empty_like(x)
+        took = []
+        for i in range(12):
+            a, b = (torch.cuda.Event(enable_timing=True) for _ in range(2))
+            a.record()
+            ops.logits_process(x, bias_ids=ids, bias=bias, out=out)
+            b.record()
+            b.synchronize()
+            took.append(a.elapsed_time(b))
+        times.append(sorted(took)[4])
+    assert times[1] <= 10 * times[0] + 0.1, times
