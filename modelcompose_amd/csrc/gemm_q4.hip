@@ -347,7 +347,8 @@ __global__ __launch_bounds__(256) void quantize_q4_kernel(const bf16_t* w, int64
 #pragma unroll
     for (int j = 0; j < 8; ++j) { const float f = (float)v[j]; lo = fminf(lo, f); hi = fmaxf(hi, f); odd |= !(fabsf(f) < INFINITY); }
     for (int o = (1 << gshift) / 16; o > 0; o >>= 1) { lo = fminf(lo, __shfl_xor(lo, o, 64)); hi = fmaxf(hi, __shfl_xor(hi, o, 64)); odd |= __shfl_xor(odd, o, 64); }
-    const float s = odd ? __uint_as_float(0x7fc00000u) : (float)(bf16_t)(zeros ? (hi - lo) / 15.f : fmaxf(hi, -lo) / 7.f);
+    const float range = hi - lo < INFINITY ? (hi - lo) / 15.f : hi / 15.f - lo / 15.f;       // (the largest numbers of both signs: finite all the same)
+    const float s = odd ? __uint_as_float(0x7fc00000u) : (float)(bf16_t)(zeros ? range : fmaxf(hi, -lo) / 7.f);
     const float z = zeros ? fminf(fmaxf(s > 0.f ? rintf(-lo / s) : 0.f, 0.f), 15.f) : 8.f;
     uint32_t out = 0;
 #pragma unroll

@@ -912,3 +912,19 @@ def test_repeated_biases_cost_about_what_different_ones_do():
             took.append(a.elapsed_time(b))
         times.append(sorted(took)[4])
     assert times[1] <= 10 * times[0] + 0.1, times
+
+
+def test_quantize_q4_of_the_largest_weights():
+    """A range that passes fp32 (the largest numbers of either sign in a group) still has a finite scale."""
+    from modelcompose_amd import ops
+    g = _gen(71)
+    top = torch.finfo(_st()).max
+    w = _rand(g, 6, 128)
+    w[1, 3], w[1, 40], w[1, 60] = top, -top, top / 2
+    w[2, 3], w[2, 4] = top, -top
+    w[3, 32:64] = top
+    q = ops.quantize_q4(w.cuda(), 32, symmetric=False)
+    s, z = q.scales.cpu().double().repeat_interleave(32, 1), q.zeros.cpu().double().repeat_interleave(32, 1)
+    assert torch.isfinite(s).all()
+    codes = torch.stack([q.codes.cpu() & 15, q.codes.cpu() >> 4], -1).view(6, 128).double()
+    assert (((codes - z) * s - w.double()).abs() <= s * (0.5 + 16 * _half() + 1e-6)).all()
