@@ -725,7 +725,7 @@ def quantize_q4(w: torch.Tensor, group: int = 128, symmetric: bool = True, bias:
     if w.dim() != 2 or group not in (32, 64, 128) or w.shape[0] == 0 or w.shape[1] == 0 or w.shape[1] % group:
         raise ValueError(f"weight must be 2-D [N, K] with K a multiple of the group (32, 64 or 128), got {tuple(w.shape)} and {group}")
     if w.stride(1) != 1 or w.stride(0) % 8 or w.stride(0) < w.shape[1] or w.data_ptr() % 16:
-        w = w.contiguous()
+        w = w.clone(memory_format=torch.contiguous_format)      # (contiguous() keeps a contiguous weight at its odd address)
     N, K = w.shape
     codes = torch.empty(N, K // 2, dtype=_U8, device=w.device)
     scales = torch.empty(N, K // group, dtype=BF16, device=w.device)

@@ -928,3 +928,15 @@ def test_quantize_q4_of_the_largest_weights():
     assert torch.isfinite(s).all()
     codes = torch.stack([q.codes.cpu() & 15, q.codes.cpu() >> 4], -1).view(6, 128).double()
     assert (((codes - z) * s - w.double()).abs() <= s * (0.5 + 16 * _half() + 1e-6)).all()
+
+
+def test_quantize_q4_of_a_weight_at_an_odd_address():
+    from modelcompose_amd import ops
+    w = _rand(_gen(72), 6, 128).cuda()
+    q = ops.quantize_q4(w, 32, symmetric=False)
+    odd = torch.zeros(6 * 128 + 8, dtype=_st(), device="cuda")[1:1 + 6 * 128].view(6, 128)
+    odd.copy_(w)
+    for v in (odd, odd[1:, :64], odd.t().contiguous().t()):
+        p, r = ops.quantize_q4(v, 32, symmetric=False), ops.quantize_q4(v.clone(memory_format=torch.contiguous_format), 32, symmetric=False)
+        assert torch.equal(p.codes, r.codes) and torch.equal(p.scales, r.scales) and torch.equal(p.zeros, r.zeros)
+    assert torch.equal(ops.quantize_q4(odd, 32, symmetric=False).codes, q.codes)
