@@ -940,3 +940,37 @@ def test_quantize_q4_of_a_weight_at_an_odd_address():
         p, r = ops.quantize_q4(v, 32, symmetric=False), ops.quantize_q4(v.clone(memory_format=torch.contiguous_format), 32, symmetric=False)
         assert torch.equal(p.codes, r.codes) and torch.equal(p.scales, r.scales) and torch.equal(p.zeros, r.zeros)
     assert torch.equal(ops.quantize_q4(odd, 32, symmetric=False).codes, q.codes)
+
+
+def test_attention_of_decode_steps_against_64_bits():
+    """Six steps of the loop: each step's projection, the key and value it appends, where it appends them, and its attention over its own cache."""
+    from modelcompose_amd import ops
+    st = _Step(9)
+    B, H, Hkv, D, S, V = st.dims
+    qkv_w = st.w["qkv"]
+    i32 = lambda t: torch.as_tensor(t, dtype=torch.int32).cuda()
+    cache = (st.cache.k, st.cache.k_scale, st.cache.v, st.cache.v_scale)
+    for _ in range(6):
+        before, x = [t.cpu().clone() for t in cache], st.embed[st.ids]
+        _, a = st()
+        lens = st.lens.cpu()
+        rows = ops.linear_q4(x, qkv_w)
+        ref, mag = q4_ref(x.cpu(), qkv_w.codes.cpu(), qkv_w.scales.cpu(), None, qkv_w.group)
+        near(rows, ref, _stored(ref) + (H * D + 16) * U * mag + 1e-30)
+        y = rows.cpu().float().view(B, H + 2 * Hkv, D)
+        want = before
+        for b in range(B):
+            t = int(lens[b]) - 1
+            for i, part in ((0, rotate(y[b, H:H + Hkv], st.cos[t].cpu(), st.sin[t].cpu())), (2, y[b, H + Hkv:])):
+                c, s = quantise(part, "e4m3")
+                want[i].view(torch.uint8)[b, :, t] = c.view(torch.uint8)
+                want[i + 1][b, :, t] = s
+        for got, ref in zip(cache, want):
+            got = got.cpu()
+            assert torch.equal(got.view(torch.uint8) if got.dim() == 4 else got, ref.view(torch.uint8) if ref.dim() == 4 else ref)
+        q16 = torch.zeros(B, H * D, dtype=_st(), device="cuda")
+        trash = [torch.zeros(B, Hkv, S, D, dtype=_st(), device="cuda") for _ in range(2)]
+        ops.rope_kv(rows, i32(range(B)), i32(lens - 1), i32([0] * B), st.cos, st.sin, q16, *trash, H, Hkv, D, 1, S)
+        q = rotate(y[:, :H].double(), st.cos[lens.long() - 1].cpu().double()[:, None], st.sin[lens.long() - 1].cpu().double()[:, None])
+        near(q16.view(B, H, D), q, _stored(q) + 4 * U * y[:, :H].double().abs().amax(-1, keepdim=True))
+        near(a.view(B, H, D), *attend(q16.cpu().double().view(B, H, D), want, lens, 1 / math.sqrt(D)))
