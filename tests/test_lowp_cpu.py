@@ -128,3 +128,42 @@ def test_wrappers_refuse_host_tensors():
         ops.linear_q4(z(1, 64, dtype=st), None)
     with pytest.raises(ValueError, match="no CPU fallback"):
         ops.attn_decode8(z(1, 1, 64, dtype=st), None)
+
+
+# ---- what the bounds of the 4-bit linears' sums reject -------------------------------------------------------------------------------
+def _q4_sum(x, codes, scales, zeros, group, group_dtype=torch.float32, sum_dtype=torch.float32, drop=0):
+    """linear_q4's arithmetic in torch: fp32 sums per group, scaled, added up - with the group sums or the running sum rounded to fewer bits, or the last `drop` columns left out."""
+    from lowp_bounds import split
+    N, G = scales.shape
+    q, s = split(codes).float().view(N, G, group), scales.float()
+    z = torch.full_like(s, 8.0) if zeros is None else zeros.float()
+    x = x.float().clone()
+    if drop:
+        x[:, -drop:] = 0
+    xg, y = x.view(len(x), G, group), torch.zeros(len(x), N)
+    for g in range(G):
+        a = (xg[:, g] @ q[:, g].t() - xg[:, g].sum(1, keepdim=True) * z[:, g]).to(group_dtype).float()
+        y = (y + a * s[:, g]).to(sum_dtype).float()
+    return y.double()
+
+
+@pytest.mark.parametrize("M", [1, 16, 48])
+@pytest.mark.parametrize("N,K,group,zeros", [(33, 11008, 128, False), (250, 4096, 128, True), (129, 2752, 64, True), (40, 544, 32, False)])
+def test_bounds_of_the_4_bit_sums_reject_what_they_should(M, N, K, group, zeros):
+    from lowp_bounds import q4_sums, whole_numbers
+    g = torch.Generator().manual_seed(N * 41 + M)
+    codes = torch.randint(0, 256, (N, K // 2), generator=g).to(torch.uint8)
+    scales = (torch.rand(N, K // group, generator=g) * 0.01 + 0.001).bfloat16()
+    z = torch.randint(0, 16, (N, K // group), generator=g).to(torch.uint8) if zeros else None
+    x = torch.randn(M, K, generator=g).bfloat16() + 0.25
+    ref, bound = q4_sums(x, codes, scales, z, group)
+    inside = lambda **kw: bool(((_q4_sum(x, codes, scales, z, group, **kw) - ref).abs() <= bound).all())
+    wrong = (dict(group_dtype=torch.bfloat16), dict(sum_dtype=torch.bfloat16), dict(drop=1), dict(drop=8))
+    assert inside()
+    for kw in wrong:
+        assert not inside(**kw), kw
+    x, codes, scales, z = whole_numbers(g, M, N, K, group, zeros, torch.bfloat16)
+    ref = q4_sums(x, codes, scales, z, group)[0]
+    assert torch.equal(_q4_sum(x, codes, scales, z, group), ref)
+    for kw in wrong:
+        assert not torch.equal(_q4_sum(x, codes, scales, z, group, **kw), ref), kw

@@ -974,3 +974,21 @@ def test_attention_of_decode_steps_against_64_bits():
         q = rotate(y[:, :H].double(), st.cos[lens.long() - 1].cpu().double()[:, None], st.sin[lens.long() - 1].cpu().double()[:, None])
         near(q16.view(B, H, D), q, _stored(q) + 4 * U * y[:, :H].double().abs().amax(-1, keepdim=True))
         near(a.view(B, H, D), *attend(q16.cpu().double().view(B, H, D), want, lens, 1 / math.sqrt(D)))
+
+
+@pytest.mark.parametrize("M", [1, 16, 17, 48, 64])
+@pytest.mark.parametrize("N,K,group,zeros", [(33, 11008, 128, False), (250, 4096, 128, True), (129, 2752, 64, True), (40, 544, 32, False), (4111, 9088, 128, True), (8208, 5248, 128, True),
+                                             (8240, 1056, 32, True), (4300, 2048, 64, False)])
+def test_linear_q4_sums_are_kept_in_fp32(M, N, K, group, zeros):
+    """Within a bound of the group sums' and the running sum's own fp32 roundings, and exact where these are."""
+    from lowp_bounds import q4_sums, whole_numbers
+    from modelcompose_amd import ops
+    g = _gen(N * 41 + M)
+    codes, scales, z = random_q4(g, N, K, group, zeros)
+    x = _rand(g, M, K) + 0.25
+    cu = lambda t: None if t is None else t.cuda()
+    y = ops.linear_q4(x.cuda(), ops.Q4Weight(cu(codes), cu(scales), cu(z)), out_f32=True)
+    near(y, *q4_sums(x, codes, scales, z, group))
+    x, codes, scales, z = whole_numbers(g, M, N, K, group, zeros, _st())
+    y = ops.linear_q4(x.cuda(), ops.Q4Weight(cu(codes), cu(scales), cu(z)), out_f32=True)
+    assert torch.equal(y.cpu().double(), q4_ref(x, codes, scales, z, group)[0])
