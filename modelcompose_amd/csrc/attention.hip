@@ -856,8 +856,8 @@ __global__ __launch_bounds__(256, UN == 4 ? 4 : 2) void attn_decode_kernel(Decod
             const float qb = __shfl_xor(qa, LPK / 2, 64), kb_ = __shfl_xor(ka, LPK / 2, 64);
             const float cs = cr[i], sn = lo ? -sr[i] : sr[i];
             // lo: x*c - partner*s ; hi: x*c + partner*s.  Rounded to bf16 like the stored q / cached k of the unfused path
-            qv[i] = (float)(bf16_t)fmaf(qa, cs, (qb * sn)) * p.scale_log2e;      // = mc_rope_pair (common.h), bit for bit
-            kr[i] = (bf16_t)fmaf(ka, cs, (kb_ * sn));
+            qv[i] = (float)(bf16_t)fp32_first(fmaf(qa, cs, (qb * sn))) * p.scale_log2e;      // = mc_rope_pair (common.h), bit for bit
+            kr[i] = (bf16_t)fp32_first(fmaf(ka, cs, (kb_ * sn)));
             knew[i] = (float)kr[i];
         }
         if (blockIdx.y == 0 && wave == 0 && slot == 0) {

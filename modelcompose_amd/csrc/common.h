@@ -77,13 +77,6 @@ __device__ __forceinline__ float mc_act(float x, int act) {
     }
 }
 
-// RoPE of one pair (a, b) = (x[d], x[d + D/2]) with cos / sin of (position, d) (apply_rotary_pos_emb, multimodal_llama.py:281-295: x cos +
-// rotate_half(x) sin).  Explicit FMAs: rope_kv_kernel and the q|k|v GEMM epilogue that replaces it round identically.
-__device__ __forceinline__ void mc_rope_pair(float a, float b, float c, float s, float& o1, float& o2) {
-    o1 = fmaf(a, c, -(b * s));
-    o2 = fmaf(b, c, a * s);
-}
-
 // Philox4x32-10 (Salmon et al. 2011; constants of the Random123 distribution, pinned by its known-answer vectors in tests/test_oracle_golden.py)
 __device__ __forceinline__ void philox4(uint32_t c0, uint32_t c1, uint32_t c2, uint32_t c3, uint32_t k0, uint32_t k1, uint32_t (&out)[4]) {
 #pragma unroll
@@ -122,6 +115,22 @@ __device__ __forceinline__ float product_rounded(float a, float b) {
     float q = a * b;
     asm("" : "+v"(q));
     return q;
+}
+
+// A value on its way to the storage type, rounded to fp32 first.  Without it the half build may fuse the operation that makes the value with the conversion
+// (v_fma_mixlo_f16: one rounding), as the compiler happens to vectorise: nothing is lost by that, but two kernels that promise each other's bits have to agree.
+__device__ __forceinline__ float fp32_first(float x) {
+#if MC_STORAGE_IS_F16
+    asm("" : "+v"(x));
+#endif
+    return x;
+}
+
+// RoPE of one pair (a, b) = (x[d], x[d + D/2]) with cos / sin of (position, d) (apply_rotary_pos_emb, multimodal_llama.py:281-295: x cos +
+// rotate_half(x) sin).  Explicit FMAs: rope_kv_kernel and the q|k|v GEMM epilogue that replaces it round identically.
+__device__ __forceinline__ void mc_rope_pair(float a, float b, float c, float s, float& o1, float& o2) {
+    o1 = fp32_first(fmaf(a, c, -(b * s)));
+    o2 = fp32_first(fmaf(b, c, a * s));
 }
 
 __device__ __forceinline__ float wave_sum(float v) {

@@ -77,7 +77,7 @@ __global__ __launch_bounds__(256) void norm_kernel(const bf16_t* __restrict__ x,
             if (bias) {
                 const bf16x8 bv = *(const bf16x8*)(bias + i * 8);
 #pragma unroll
-                for (int j = 0; j < 8; ++j) o[j] = (bf16_t)((v[it][j] - mean) * rstd * (float)wv[j] + (float)bv[j]);
+                for (int j = 0; j < 8; ++j) o[j] = (bf16_t)fp32_first((v[it][j] - mean) * rstd * (float)wv[j] + (float)bv[j]);
             } else {
 #pragma unroll
                 for (int j = 0; j < 8; ++j) o[j] = (bf16_t)((v[it][j] - mean) * rstd * (float)wv[j]);
@@ -92,7 +92,7 @@ __global__ __launch_bounds__(256) void norm_kernel(const bf16_t* __restrict__ x,
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
             float r = ((float)t[j] - mean) * rstd * (float)wv[j];
-            if (bias) r += (float)bias[i * 8 + j];
+            if (bias) r = fp32_first(r + (float)bias[i * 8 + j]);
             o[j] = (bf16_t)r;
         }
         *(bf16x8*)(orow + i * 8) = o;
@@ -153,7 +153,7 @@ __global__ __launch_bounds__(256) void norm_rows_kernel(const bf16_t* __restrict
             if (bias) {
                 const bf16x8 bv = *(const bf16x8*)(bias + i * 8);
 #pragma unroll
-                for (int j = 0; j < 8; ++j) o[j] = (bf16_t)((v[it][j] - mean) * rstd * (float)wv[j] + (float)bv[j]);
+                for (int j = 0; j < 8; ++j) o[j] = (bf16_t)fp32_first((v[it][j] - mean) * rstd * (float)wv[j] + (float)bv[j]);
             } else {
 #pragma unroll
                 for (int j = 0; j < 8; ++j) o[j] = (bf16_t)((v[it][j] - mean) * rstd * (float)wv[j]);
@@ -232,7 +232,7 @@ __global__ __launch_bounds__(256) void add_norm_rows_kernel(const bf16_t* __rest
             const bf16x8 wv = *(const bf16x8*)(w + i * 8), bv = *(const bf16x8*)(bias + i * 8);
             bf16x8 o;
 #pragma unroll
-            for (int j = 0; j < 8; ++j) o[j] = (bf16_t)((v[it][j] - mean) * rstd * (float)wv[j] + (float)bv[j]);
+            for (int j = 0; j < 8; ++j) o[j] = (bf16_t)fp32_first((v[it][j] - mean) * rstd * (float)wv[j] + (float)bv[j]);
             *(bf16x8*)(orow + i * 8) = o;
         }
     }

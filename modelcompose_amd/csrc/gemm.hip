@@ -123,7 +123,7 @@ __device__ __forceinline__ bf16x4 epilogue_vals4(const Epilogue& e, float a, int
     }
     if (RESC == 1 || (RESC == -1 && has_res)) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) r[i] += e.beta * (float)res[i];
+        for (int i = 0; i < 4; ++i) r[i] = fp32_first(r[i] + e.beta * (float)res[i]);
     }
     return (bf16x4){(bf16_t)r[0], (bf16_t)r[1], (bf16_t)r[2], (bf16_t)r[3]};
 }

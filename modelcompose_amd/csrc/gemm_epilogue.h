@@ -48,7 +48,7 @@ __device__ __forceinline__ void epilogue_store4(const Epilogue& e, int m, int n,
     if (e.residual) {
         bf16x4 b = *(const bf16x4*)(e.residual + (int64_t)m * e.ldr + n);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) r[i] += e.beta * (float)b[i];
+        for (int i = 0; i < 4; ++i) r[i] = fp32_first(r[i] + e.beta * (float)b[i]);
     }
     if (e.out_f32) {
         f32x4 o = {r[0], r[1], r[2], r[3]};

@@ -117,10 +117,10 @@ __global__ __launch_bounds__(256) void kv8_read_kernel(Cache c, const int32_t* k
                 float f[4];
                 kv8_unpack4<FMT>(w[0], f);
 #pragma unroll
-                for (int j = 0; j < 4; ++j) o[j] = (bf16_t)(f[j] * s);
+                for (int j = 0; j < 4; ++j) o[j] = (bf16_t)fp32_first(f[j] * s);
                 kv8_unpack4<FMT>(w[1], f);
 #pragma unroll
-                for (int j = 0; j < 4; ++j) o[4 + j] = (bf16_t)(f[j] * s);
+                for (int j = 0; j < 4; ++j) o[4 + j] = (bf16_t)fp32_first(f[j] * s);
             }
             *(bf16x8*)((kv ? v_out : k_out) + ((int64_t)bh * n + pos) * D + d) = o;
         }

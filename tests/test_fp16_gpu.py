@@ -85,3 +85,71 @@ def test_fp16_full_depth_eight_rows_against_the_fp32_oracle():
     # a flipped argmax is a near-tie of the oracle itself: its top-2 margin is below twice the measured error (in logit units)
     for m in tf["disagreement_margins"]:
         assert m <= 2 * rep["hip_vs_fp32_oracle"]["max"] * rep["logit_scale"], (m, rep["hip_vs_fp32_oracle"]["max"], rep["logit_scale"])
+
+
+def _child(code, *args):
+    if not torch.cuda.is_available():
+        pytest.skip("needs a GPU")
+    r = subprocess.run([sys.executable, "-c", code, *args], capture_output=True, text=True, timeout=300, cwd=ROOT, env=dict(os.environ, MC_STORAGE_DTYPE="fp16"))
+    assert r.returncode == 0, (r.stdout[-3000:], r.stderr[-2000:])
+    return r.stdout
+
+
+_DIGESTS = """
+import hashlib, json, sys
+import torch
+sys.path.insert(0, ".")
+from modelcompose_amd import _lib
+from modelcompose_amd import ops
+assert ops.BF16 == torch.float16 and _lib.lib().mc_storage_dtype() == 2
+g = torch.Generator().manual_seed(3)
+r = lambda *s, k=1.0: (torch.randn(*s, generator=g) * k).half().cuda()
+sha = lambda t: hashlib.sha256(t.contiguous().view(torch.uint8).cpu().numpy().tobytes()).hexdigest()[:16]
+x, w, dy = r(333, 4096), r(4096), r(333, 4096)
+big, h = r(48, 4096), r(8192, 4096, k=0.02)
+out = {"rmsnorm": ops.rmsnorm(x, w, 1e-6), "layernorm_bwd": ops.layernorm_bwd(x[:, :1280].contiguous(), w[:1280].contiguous(), dy[:, :1280].contiguous(), 1e-5)}
+for a in ("gelu", "quick_gelu", "silu"):
+    out["act " + a] = ops.act(x, a)
+    out["act " + a + " bwd"] = ops.act(x, a, dy=dy)
+pw = ops.pack_weight(h)
+for M in (1, 16, 48):
+    out["linear_ex swiglu %d" % M] = ops.linear_ex(big[:M], pw, swiglu=True, rms_eps=1e-6)
+first = lambda t: t[0] if isinstance(t, (tuple, list)) else t
+print(json.dumps({k: sha(first(v)) for k, v in out.items()}))
+"""
+
+
+# recorded from the half library as it was before the build left out packed fp32 instructions
+_BEFORE = {"rmsnorm": "c408e0ad3530bf87", "layernorm_bwd": "da6e18fccf6a9400", "act gelu": "a320e95056cde187", "act gelu bwd": "2d030471335e4da9", "act quick_gelu": "ec93855894c391fc",
+           "act quick_gelu bwd": "236d7ed5238e43cd", "act silu": "fb25749713a11b96", "act silu bwd": "d47b0feacf87fc30", "linear_ex swiglu 1": "249df3687d5665c0",
+           "linear_ex swiglu 16": "102434fb26c9393b", "linear_ex swiglu 48": "689321a757f71bb4"}
+
+
+def test_fp16_results_are_those_of_before():
+    """Bit for bit: where an operation and the rounding of its result to half were one instruction (v_fma_mixlo_f16), they still are - the build flags do not forbid it;
+    what two kernels promise each other is rounded to fp32 first in the source (fp32_first), in both."""
+    got = json.loads(_child(_DIGESTS).splitlines()[-1])
+    assert got == _BEFORE, {k: v for k, v in got.items() if v != _BEFORE[k]}
+
+
+_PYTEST = """
+import sys
+import torch
+if sys.argv[1] == "half":                       # (tests that name their tensors' type)
+    torch.bfloat16, torch.Tensor.bfloat16 = torch.float16, torch.Tensor.half
+import pytest
+sys.exit(pytest.main(["-q", "-x", "--timeout", "120", "--timeout-method", "thread", "-p", "no:cacheprovider", *sys.argv[2:]]))
+"""
+
+
+def test_fp16_kernels_that_promise_each_others_bits():
+    """The query / key / value projection with rotation in its epilogue against the separate kernels, the fused add + LayerNorm against the two, the row factor of the stored
+    rows against the separate pass, on the half library."""
+    out = _child(_PYTEST, "half", "tests/test_ops_gpu.py", "tests/test_encoders_gpu.py", "-k", "qkv_projection_with_rope_scatter or gemm_rms_out_factor or fused_add_layernorm")
+    assert "passed" in out and "failed" not in out
+
+
+def test_fp16_low_precision_operators():
+    """The 8-bit cache, the 4-bit linears and the logits processor on the half library: the whole of their tests."""
+    out = _child(_PYTEST, "-", "tests/test_lowp_gpu.py")
+    assert "passed" in out and "failed" not in out
