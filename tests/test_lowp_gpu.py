@@ -992,3 +992,32 @@ def test_linear_q4_sums_are_kept_in_fp32(M, N, K, group, zeros):
     x, codes, scales, z = whole_numbers(g, M, N, K, group, zeros, _st())
     y = ops.linear_q4(x.cuda(), ops.Q4Weight(cu(codes), cu(scales), cu(z)), out_f32=True)
     assert torch.equal(y.cpu().double(), q4_ref(x, codes, scales, z, group)[0])
+
+
+@pytest.mark.parametrize("M", [1, 7, 40])
+def test_linear_q4_of_a_row_of_nan(M):
+    """A sequence that has become NaN stays NaN and leaves the others alone, at about the cost of any other row."""
+    from modelcompose_amd import ops
+    g = _gen(81)
+    codes, scales, z = random_q4(g, 4100, 4096, 128, True)
+    w = ops.Q4Weight(codes.cuda(), scales.cuda(), z.cuda())
+    x = _rand(g, M, 4096).cuda()
+    clean = ops.linear_q4(x, w)
+    bad = x.clone()
+    bad[M // 2] = math.nan
+    y = ops.linear_q4(bad, w)
+    assert torch.isnan(y[M // 2]).all()
+    rest = [m for m in range(M) if m != M // 2]
+    assert torch.equal(y[rest], clean[rest])
+    times = []
+    for v in (x, bad):
+        took = []
+        for _ in range(12):
+            a, b = (torch.cuda.Event(enable_timing=True) for _ in range(2))
+            a.record()
+            ops.linear_q4(v, w, out=y)
+            b.record()
+            b.synchronize()
+            took.append(a.elapsed_time(b))
+        times.append(sorted(took)[4])
+    assert times[1] <= 2 * times[0] + 0.05, times
