@@ -1,6 +1,8 @@
 import json
+import multiprocessing.context
 import os
 import sys
+import time
 
 import numpy as np
 import pytest
@@ -12,8 +14,22 @@ if ROOT not in sys.path:
 GOLDEN = os.path.join(ROOT, "tests", "golden")
 
 
+class _Lingering(multiprocessing.context.SpawnProcess):
+    """A spawned worker that stays until the tensors it put on a queue have been fetched.  They are handed over by a thread of the worker, and one that ends right after its put()
+    may take that thread with it, between two steps of the hand-over (a matter of milliseconds, decided by when the collector of either process runs)."""
+
+    def run(self):
+        super().run()
+        from multiprocessing.resource_sharer import _resource_sharer
+        empty, end = 0, time.monotonic() + 30
+        while empty < 5 and time.monotonic() < end:
+            time.sleep(0.1)
+            empty = 0 if _resource_sharer._cache else empty + 1
+
+
 def pytest_configure(config):
     config.addinivalue_line("markers", "gpu: needs a real MI355X (run with -m gpu on the GPU box)")
+    multiprocessing.context.SpawnContext.Process = _Lingering
 
 
 def pytest_sessionstart(session):
