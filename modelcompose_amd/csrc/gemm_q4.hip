@@ -318,12 +318,15 @@ void q4_launch_g(const Q4Params& p, hipStream_t s) {
     else q4_launch_z<W, MB, R, U, UX, 5>(p, s);
 }
 
-// R blocks of 16 columns per workgroup: enough to bring the workgroups down to one per CU, up to 3 (x is read once per workgroup: 48 x 12288 x 4096 takes 25 us with R = 1, 23
-// with 2, 19 with 3; 1 x 4096 x 4096, whose 256 blocks just fill the chip, 5.2, 6.7 and 8.5).  Waves per workgroup, a function of N alone because it decides the order of the
-// sums: 8 up to 512 blocks, where longer chains leave the chip idle (1 x 4096 x 4096: 5.2 against 6.2 us), 4 above, where shorter ones spend their time starting and
-// ending (8 x 32000 x 4096: 22 against 34 us).
-// Above 16 rows a SIMD has one wave, and its time is its own instructions': of the 18 us of 48 x 12288 x 4096 the packing of x takes 3, the sums over the waves and the stores 2, the
-// loop 8 without any load and 13 with them.  One wave per row block instead (three a SIMD, codes converted three times): 22 us; x or codes requested two blocks ahead: 18.
+// Times with weights in turn, none found in the last-level cache, as a decode step meets them (a single 4096 x 4096 weight replayed from it takes 4.9 us instead of 6.6).
+// R blocks of 16 columns per workgroup: enough to bring the workgroups down to one per CU, up to 3 (x is read once per workgroup: 48 x 12288 x 4096 takes 24.1 us with R = 1, 21.7
+// with 2, 19.2 with 3, 48 x 22016 x 4096 40.8, 31.0 and 27.5; 1 x 4096 x 4096, whose 256 blocks just fill the chip, 6.6, 8.4 and 10.4).  Waves per workgroup, a function of N alone
+// because it decides the order of the sums: 8 up to 512 blocks, where longer chains leave the chip idle (48 x 4096 x 11008: 23.7 against 25.8 us, 48 x 4096 x 4096 11.9 against
+// 12.4, 1 x 4096 x 4096 either way 6.6), 4 above, where shorter ones spend their time starting and ending (8 x 32000 x 4096: 22.9 against 29.3 us, 48 x 22016 x 4096 27.5 against 31.8;
+// 48 x 12288 x 4096, at the border, 19.2 against 18.5).
+// Above 16 rows a SIMD has one wave, and its time is its own instructions' and what its loads leave open: of 17 us of 48 x 12288 x 4096 with the weight in the cache the packing of x
+// takes 3, the sums over the waves and the stores 2, the loop 8 without any load and 13 with them.  One wave per row block instead (three a SIMD, codes converted three
+// times): 22 us; x or codes requested two blocks ahead: 18.
 template <int MB>
 void q4_launch(const Q4Params& p, hipStream_t s) {
     const int tiles = (p.N + 15) / 16;

@@ -146,8 +146,8 @@ __device__ __forceinline__ int attn8_len(const AttnParams8& p, int b) {
     return max(0, min(n, p.c.S));
 }
 
-// Keys of one partial: a function of the sequence's own length, so that short sequences still spread over many workgroups (1 x 2809 keys: 13 us with 512, 18 with 1024)
-// and long ones are not ground into partials (8 x 32768 keys: 129 us with 512, 94 with 2048).
+// Keys of one partial: a function of the sequence's own length, so that short sequences still spread over many workgroups (1 x 2809 keys: 12.6 us with 512, 17.3 with 1024;
+// 48 x 2809, where it does not matter, 146 and 144) and long ones are not ground into partials (8 x 32768 keys: 97 us with 512, 92 with 2048).
 __host__ __device__ inline int attn8_chunk(int n) { return n <= 4096 ? 512 : n <= 16384 ? 1024 : 2048; }
 typedef float f32x4_u __attribute__((ext_vector_type(4), aligned(4)));
 typedef uint32_t u32x2_u __attribute__((ext_vector_type(2), aligned(1)));
@@ -594,7 +594,7 @@ int check_rope(const void* qkv, int64_t ld, const float* cos_table, const float*
     return 0;
 }
 
-// 4096 workgroups fill the chip five times over, while there are chunks to hand out (48 x 2809 keys: 160 us with 4608 workgroups, 167 with 1536, 169 with 9216)
+// 4096 workgroups fill the chip five times over, while there are chunks to hand out (48 x 2809 keys: 146 us with 4608 workgroups, 152 with 1536, 157 with 9216)
 int attn8_launch(AttnParams8& p, const mc_kv8_cache* c, hipStream_t s, const char* who) {
     const int chunks = attn8_max_parts(c->S);
     p.G = p.H / c->Hkv;
@@ -604,7 +604,7 @@ int attn8_launch(AttnParams8& p, const mc_kv8_cache* c, hipStream_t s, const cha
     MC_CHECK_ARG(c->B == 1 || p.o_sb >= (int64_t)p.H * c->D, "%s: output rows overlap", who);
     MC_CHECK_ARG(wgs < (1LL << 23) && (int64_t)c->B * p.H < (1LL << 23), "%s: B * H = %lld is too large for one launch", who, (long long)c->B * p.H);
     // up to two chunks: one workgroup takes both and joins them itself.  Launched one call at a time the second launch costs more than it saves (5 x 517 keys: 14.8
-    // against 17.4 us a call; replayed from a graph 12.2 against 10.1)
+    // against 17.4 us a call); replayed from a graph it would pay (12.4 against 10.3)
     const int want = (int)((4096 + wgs - 1) / wgs), split = chunks <= 2 ? 1 : want < chunks ? want : chunks;
     p.self_combine = split == 1;
     const dim3 grid((unsigned)wgs, split);
