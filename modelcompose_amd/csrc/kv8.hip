@@ -244,8 +244,9 @@ __device__ __forceinline__ void attn8_append(const AttnParams8& p, int b, int hk
 // the same head; with row r of half t standing for key 8 (r >> 2) + 4 t + (r & 3), lane (c, g) ends up with the scores of keys 8 g .. 8 g + 7 of head
 // c & 7 - exactly the layout in which the next product O^T = V^T P^T wants its B operand, so the probabilities never leave the lane.  They
 // enter that product as bfloat16, whose 8 significant bits are three parts of the fp32 weight w = p * v_scale = hi + mid + low, exactly: hi in columns 0 .. 7 and mid in columns
-// 8 .. 15 of one operand, low in columns 0 .. 7 of a second (bfloat16 also in the half-precision build: w has a wide range).  Two
-// parts (an error of 2^-17, nine times that of fp32 arithmetic in the sum) took 144.0 us where three take 145.5 (48 x 2809 keys), 12.4 against 12.6 (1 x 2809).
+// 8 .. 15 of one operand, low in columns 0 .. 7 of a second (bfloat16 also in the half-precision build: w has a wide range).  Of
+// the 16-bit outputs of 48 x 2809 keys 0.6 in a thousand are not the rounded exact value (the same in fp32 in torch: 1.3); with two parts, off by 2^-17, it was 2.5, in
+// 144.0 us where three take 145.5 (1 x 2809: 12.4 against 12.6).
 // V^T's operand needs 8 keys of one element per lane: the bytes of two keys' rows are paired by v_perm.
 //
 // A workgroup of 4 waves takes chunks (attn8_chunk keys) blockIdx.y, + gridDim.y, ..; wave w the 32-key tiles w, w + 4, .. of a chunk, from a fresh (m, l, acc); the
